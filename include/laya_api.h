@@ -226,6 +226,45 @@ int laya_b200_gemm_splitk_noalloc(const void* A, const void* W, void* out, float
                                   const float* cos_t, const float* sin_t, const int* pos, int rope_cols,
                                   int geglu_I, int splits, void* stream, int sync);
 
+/* ----------------------------------------------------------------- layer operators
+ * A transformer layer's norm, matrix product and attention on caller-owned device memory (additions,
+ * no counterpart in the reference). They share these rules. Pointers name memory of the current
+ * device; a pointer that no device or another device owns is refused (-2). Element types are
+ * LAYA_BF16, LAYA_F16, LAYA_F32 and LAYA_E4M3 (8 bits: 4 exponent and 3 mantissa bits, largest value
+ * 448). ld* are distances between rows in elements; rows must not overlap. Outputs are written inside
+ * their rows and columns only. Every call launches on `stream` (NULL: the default stream), keeps
+ * nothing of a call and may overlap other calls; it can be captured into a graph once any layer
+ * operator has run on the device outside a capture (else -8), with sync 0. sync != 0 waits for the
+ * GPU. Returns 0, -1 no device, -2 an argument is refused (nothing was launched), -4 set-up failed,
+ * -5 a launch failed, -6 the GPU reported an error, -8 as above, -100-code when a kernel gave up
+ * (sync; see laya_b200_kernel_error). */
+enum { LAYA_BF16 = 0, LAYA_F16 = 1, LAYA_F32 = 2, LAYA_E4M3 = 3 };
+
+/* Norm of a residual sum, per row of D elements (1 <= D <= 16384):
+ *   h = x + resid;  z = h - center * mean(h);  y = z / sqrt(mean(z^2) + eps) * w + b
+ * center 0: root-mean-square norm, 1: LayerNorm. resid (or NULL) and x are LAYA_BF16 / F16 / F32, w
+ * and b (or NULL) fp32. sum (or NULL) receives h in sum_type; it may be x or resid itself (the same
+ * pointer, type and stride). y is computed from h in fp32, before h is rounded to sum_type. out_type
+ * LAYA_BF16 / F16 / F32: out = y. LAYA_E4M3: scale[row] = max(max|y| / 448, 2^-126) and out = y /
+ * scale[row], rounded to nearest even; scale is given exactly with this type. A row with a NaN has NaN
+ * in its scale. rows 0 does nothing. */
+int laya_b200_norm(const void* x, int x_type, long long ldx, const void* resid, int resid_type, long long ldr,
+                   void* sum, int sum_type, long long lds, const float* w, const float* b, float eps, int center,
+                   void* out, int out_type, long long ldo, float* scale, int rows, int D, void* stream, int sync);
+
+/* Matrix product with everything after it in one pass (W as torch.nn.Linear stores it):
+ *   out[m][n] = act(a_scale[m] * w_scale[n] * sum_k A[m][k] W[n][k] + bias[n]) + resid[m][n]
+ * A [M][K] and W [N][K] both LAYA_BF16, LAYA_F16 or LAYA_E4M3 (ab_type), sums in fp32; a_scale [M],
+ * w_scale [N] (with any ab_type; 1 where NULL) and bias [N] (or NULL) fp32. act 0 none, 1 ReLU, 2 GELU
+ * (erf), 3 SiLU. out_type LAYA_BF16 / F16 / F32 is also resid's; resid (or NULL) may be out itself (the
+ * same pointer and stride). Any M, N, K up to 2^24 (K >= 1; M or N 0 does nothing). Rows of A and W start
+ * on 16 bytes: their addresses and strides in bytes are multiples of 16; what storage holds past
+ * column K is not used. out, resid and the vectors may have any alignment of their type. The sums'
+ * order depends only on the sizes and types. */
+int laya_b200_linear(const void* A, long long lda, const void* W, long long ldw, int ab_type, const float* a_scale,
+                     const float* w_scale, const float* bias, int act, const void* resid, long long ldr, void* out,
+                     int out_type, long long ldo, int M, int N, int K, void* stream, int sync);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,6 +34,7 @@ def load_lib(path: str = LIB_PATH) -> ctypes.CDLL:
         raise RuntimeError("liblaya_b200.so not built (run python -m layamd_b200.build): %s" % path)
     L = ctypes.CDLL(path)
     vp, i, f, d = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_double
+    ll = ctypes.c_longlong
     sig = {
         "laya_create": (vp, [ctypes.c_char_p]),
         "laya_forward_batch": (i, [vp, i, _IP, _IP, _IP, _IP, _IP, _FP, _FP]),
@@ -69,6 +70,8 @@ def load_lib(path: str = LIB_PATH) -> ctypes.CDLL:
         "laya_b200_kernel_error": (i, [i]),
         "laya_pack_check": (i, [i, i, i, i, i, i, _IP, _IP, _IP, _IP, _IP, i]),
         "laya_debug_bounds_build": (i, []),
+        "laya_b200_norm": (i, [vp, i, ll, vp, i, ll, vp, i, ll, vp, vp, f, i, vp, i, ll, vp, i, i, vp, i]),
+        "laya_b200_linear": (i, [vp, ll, vp, ll, i, vp, vp, vp, i, vp, ll, vp, i, ll, i, i, i, vp, i]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -1,0 +1,140 @@
+// C entries of the layer operators on caller-owned device memory (laya_b200_norm, laya_b200_linear,
+// laya_b200_attention_varlen): the checks of their arguments, the per-device set-up and the launches.
+// They are additions to the reference ABI.
+//
+// Every argument that can be checked on the host is checked before anything is launched; memory that
+// another device, or no device, holds is refused. No entry keeps anything of a call: outputs and
+// workspaces belong to the caller, so calls may overlap on any streams, and a captured call replays.
+#include <cmath>
+#include <cstdio>
+#include <initializer_list>
+#include <mutex>
+
+#include "kernels.h"
+#include "laya_api.h"
+#include "layer_ops.h"
+
+namespace {
+using namespace laya;
+
+constexpr int kMaxDevices = 64;
+struct Device {
+  bool ready = false;
+  int sms = 0;
+  int pairs = 0;       // co-resident CTA pairs of the matrix product
+  int* err = nullptr;  // the error word that the kernel-level entries share
+};
+std::mutex g_mu;
+Device g_dev[kMaxDevices];
+
+bool device_memory(const void* p, int dev) {
+  cudaPointerAttributes at;
+  if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev);
+}
+
+// The current device, set up, for a call on `stream` with these arrays (null ones are not given).
+// Returns 0 or the entry's error code.
+int begin(void* stream, int sync, std::initializer_list<const void*> arrays, Device* d) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  if (dev < 0 || dev >= kMaxDevices) return -4;
+  for (const void* p : arrays)
+    if (p && !device_memory(p, dev)) return -2;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &cap) != cudaSuccess) {
+    cudaGetLastError();
+    return -5;
+  }
+  if (cap != cudaStreamCaptureStatusNone && sync) return -2;  // a captured call cannot wait for its work
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (!g_dev[dev].ready) {
+    if (cap != cudaStreamCaptureStatusNone) return -8;  // set-up allocates: not inside a capture
+    if (cudaDeviceGetAttribute(&g_dev[dev].sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -4;
+    if (linear_prepare_device(&g_dev[dev].pairs) != cudaSuccess) return -4;
+    g_dev[dev].err = entry_error_word(dev);
+    if (!g_dev[dev].err) return -4;
+    g_dev[dev].ready = true;
+  }
+  *d = g_dev[dev];
+  return 0;
+}
+
+// After the launch: its error, and with `sync` the wait and the kernel's own error code.
+int finish(const char* what, cudaError_t e, void* stream, int sync, int* err) {
+  if (e != cudaSuccess) {
+    fprintf(stderr, "[laya] %s launch: %s\n", what, cudaGetErrorString(e));
+    cudaGetLastError();
+    return -5;
+  }
+  if (!sync) return 0;
+  if (cudaStreamSynchronize(static_cast<cudaStream_t>(stream)) != cudaSuccess) return -6;
+  int h = 0;
+  if (cudaMemcpy(&h, err, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -6;
+  if (!h) return 0;
+  cudaMemset(err, 0, sizeof(int));
+  return -100 - h;
+}
+
+bool is16(int t) { return t == DT_BF16 || t == DT_F16; }
+bool is_plain(int t) { return is16(t) || t == DT_F32; }
+bool is_aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
+// rows of `cols` elements that lie `ld` apart do not overlap (one row has no stride)
+bool strides_ok(int rows, int cols, long long ld) { return rows <= 1 || ld >= cols; }
+}  // namespace
+
+extern "C" int laya_b200_norm(const void* x, int x_type, long long ldx, const void* resid, int resid_type,
+                              long long ldr, void* sum, int sum_type, long long lds, const float* w, const float* b,
+                              float eps, int center, void* out, int out_type, long long ldo, float* scale, int rows,
+                              int D, void* stream, int sync) {
+  if (rows < 0 || D < 1 || D > kNormMaxD || !is_plain(x_type) || (center != 0 && center != 1)) return -2;
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return -2;
+  if ((resid && !is_plain(resid_type)) || (sum && !is_plain(sum_type))) return -2;
+  if (!is_plain(out_type) && out_type != DT_E4M3) return -2;
+  if (rows == 0) return 0;
+  if (!x || !w || !out || (out_type == DT_E4M3) != (scale != nullptr)) return -2;
+  if (!strides_ok(rows, D, ldx) || (resid && !strides_ok(rows, D, ldr)) || (sum && !strides_ok(rows, D, lds)) ||
+      !strides_ok(rows, D, ldo))
+    return -2;
+  if (!is_aligned(x, type_size(x_type)) || (resid && !is_aligned(resid, type_size(resid_type))) ||
+      (sum && !is_aligned(sum, type_size(sum_type))) || !is_aligned(out, type_size(out_type)) || !is_aligned(w, 4) ||
+      !is_aligned(b, 4) || !is_aligned(scale, 4))
+    return -2;
+  Device d;
+  if (int rc = begin(stream, sync, {x, resid, sum, w, b, out, scale}, &d)) return rc;
+  const NormArgs a{x,      ldx,        resid,    ldr,      sum,  lds, w,      b,  out, ldo, scale,
+                   x_type, resid_type, sum_type, out_type, rows, D,   center, eps};
+  return finish("norm", norm_launch(a, d.sms, static_cast<cudaStream_t>(stream)), stream, sync, d.err);
+}
+
+extern "C" int laya_b200_linear(const void* A, long long lda, const void* W, long long ldw, int ab_type,
+                                const float* a_scale, const float* w_scale, const float* bias, int act,
+                                const void* resid, long long ldr, void* out, int out_type, long long ldo, int M, int N,
+                                int K, void* stream, int sync) {
+  if (M < 0 || N < 0 || K < 1 || K > kLinearMaxDim || M > kLinearMaxDim || N > kLinearMaxDim) return -2;
+  if ((!is16(ab_type) && ab_type != DT_E4M3) || !is_plain(out_type) || act < LIN_NONE || act > LIN_SILU) return -2;
+  if (M == 0 || N == 0) return 0;
+  if (!A || !W || !out) return -2;
+  const int es = type_size(ab_type), os = type_size(out_type);
+  // operand rows start on 16 bytes (the tensor copies need it); one row has no stride of its own
+  if (M == 1 && lda < K) lda = (K * (long long)es + 15) / 16 * 16 / es;
+  if (N == 1 && ldw < K) ldw = (K * (long long)es + 15) / 16 * 16 / es;
+  if (lda < K || ldw < K || lda > kLinearMaxLd || ldw > kLinearMaxLd || (lda * es) % 16 != 0 || (ldw * es) % 16 != 0)
+    return -2;
+  if (!is_aligned(A, 16) || !is_aligned(W, 16)) return -2;
+  if (!strides_ok(M, N, ldo) || (resid && !strides_ok(M, N, ldr))) return -2;
+  if (!is_aligned(out, os) || !is_aligned(resid, os) || !is_aligned(a_scale, 4) || !is_aligned(w_scale, 4) ||
+      !is_aligned(bias, 4))
+    return -2;
+  Device d;
+  if (int rc = begin(stream, sync, {A, W, a_scale, w_scale, bias, resid, out}, &d)) return rc;
+  const LinearArgs a{A, lda, W, ldw, a_scale, w_scale, bias, resid, ldr, out, ldo, ab_type, out_type, act, M, N, K, 0};
+  return finish("linear", linear_launch(a, d.sms, d.pairs, d.err, static_cast<cudaStream_t>(stream)), stream, sync,
+                d.err);
+}

@@ -14,6 +14,7 @@
 // matrix through L2 and read each activation row block from HBM once.
 #include "common.cuh"
 #include "kernels.h"
+#include "layer_ops.h"
 #include <algorithm>
 #include <cstdio>
 
@@ -800,6 +801,23 @@ bool make_operand_map(CUtensorMap* map, const void* base, uint64_t K, uint64_t r
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
+}
+
+bool make_rows_map(CUtensorMap* map, const void* base, int type, uint64_t cols, uint64_t mid, uint64_t rows,
+                   uint64_t mid_stride, uint64_t ld, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const uint64_t es = static_cast<uint64_t>(type_size(type));
+  const CUtensorMapDataType dt = type == DT_E4M3   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : type == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  cuuint64_t dims[3] = {cols, mid, rows};
+  cuuint64_t strides[2] = {mid_stride * es, ld * es};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / es), 1, box_rows};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool make_output_map(CUtensorMap* map, const void* base, bool f32, uint64_t ld, uint64_t rows, uint64_t planes) {

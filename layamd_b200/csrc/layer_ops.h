@@ -1,0 +1,65 @@
+// Host-side launchers of the layer operators (norm.cu, linear.cu, attn_varlen.cu): one transformer
+// layer's norm, matrix product and attention on caller-owned device memory, of any size and type. They
+// serve the C entries of abi_layer.cu; the engine's own pass does not use them.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace laya {
+
+// Element types (LAYA_BF16 .. LAYA_E4M3 of the C header).
+enum DataType : int { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2, DT_E4M3 = 3 };
+constexpr int type_size(int t) { return t == DT_F32 ? 4 : t == DT_E4M3 ? 1 : 2; }
+
+// Strides (ld*) are in elements.
+struct NormArgs {
+  const void* x;
+  long long ldx;
+  const void* resid;  // or null
+  long long ldr;
+  void* sum;          // or null: h = x + resid in sum_type
+  long long lds;
+  const float* w;
+  const float* b;     // or null
+  void* out;
+  long long ldo;
+  float* scale;       // [rows], e4m3 output only
+  int x_type, resid_type, sum_type, out_type;
+  int rows, D, center;
+  float eps;
+};
+constexpr int kNormMaxD = 16384;  // 512 threads x 4 pieces x 8 elements
+cudaError_t norm_launch(const NormArgs& a, int num_sms, cudaStream_t st);
+
+enum LinearAct : int { LIN_NONE = 0, LIN_RELU = 1, LIN_GELU = 2, LIN_SILU = 3 };
+// out[m][n] = act(a_scale[m] * w_scale[n] * sum_k A[m][k] W[n][k] + bias[n]) + resid[m][n]
+struct LinearArgs {
+  const void* A;
+  long long lda;
+  const void* W;
+  long long ldw;
+  const float* a_scale;  // or null: 1
+  const float* w_scale;  // or null: 1
+  const float* bias;     // or null
+  const void* resid;     // or null; out_type
+  long long ldr;
+  void* out;
+  long long ldo;
+  int ab_type, out_type, act;
+  int M, N, K;
+  int vec_out;  // out and resid rows start on 16 bytes (set by the launcher)
+};
+cudaError_t linear_prepare_device(int* pair_clusters);
+cudaError_t linear_launch(const LinearArgs& a, int num_sms, int pair_clusters, int* err, cudaStream_t st);
+constexpr int kLinearMaxDim = 1 << 24;         // M, N, K: row and column arithmetic stays in 32 bits
+constexpr long long kLinearMaxLd = 1LL << 32;  // the tensor maps' strides stay below 2^40 bytes
+constexpr int kLinearFewRows = 16;  // most rows of the kernel for few rows
+cudaError_t linear_few_launch(const LinearArgs& a, int num_sms, cudaStream_t st);
+
+// Tensor map of rows [rows][mid][cols] (strides in elements) loaded in 128-byte-wide boxes of box_rows
+// rows with the 128-byte swizzle; defined beside the engine's operand maps.
+bool make_rows_map(CUtensorMap* map, const void* base, int type, uint64_t cols, uint64_t mid, uint64_t rows,
+                   uint64_t mid_stride, uint64_t ld, uint32_t box_rows);
+
+}  // namespace laya
