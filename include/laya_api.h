@@ -265,6 +265,33 @@ int laya_b200_linear(const void* A, long long lda, const void* W, long long ldw,
                      const float* w_scale, const float* bias, int act, const void* resid, long long ldr, void* out,
                      int out_type, long long ldo, int M, int N, int K, void* stream, int sync);
 
+/* Attention of packed sequences with masks, distance bias and capped scores. Sequence b has query rows
+ * cu_q[b] .. cu_q[b + 1] - 1 of q [rows_q][Hq][D] and key rows cu_k[b] .. cu_k[b + 1] - 1 of k and v
+ * [rows_k][Hkv][D] (device arrays of B + 1 offsets, B <= 65535); query head h uses key head h / (Hq / Hkv).
+ * Query i of lq sits at key position p = i + lk - lq: at lq = lk on its own key, with fewer queries than
+ * keys on the last ones. For key j:
+ *   s = scale * q_i . k_j;  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s -= slopes[h] * |p - j|
+ *   seen: (p - left <= j <= p + right, or j < prefix[b])  and  doc_q[i] == doc_k[j] >= 0
+ *   out_i = sum_j softmax(s)_j v_j over the keys seen, lse[i][h] = log sum_j exp(s)
+ * left, right -1: unbounded (right 0 is causal); slopes [Hq] fp32, prefix [B], doc_q [rows_q] and doc_k
+ * [rows_k] (both or neither) are device arrays or NULL; lse [rows_q][Hq] fp32 or NULL. A row that sees
+ * nothing gets 0 and lse -infinity. q, k, v, out are LAYA_BF16 or LAYA_F16, D is 64 or 128; their rows
+ * start on 16 bytes (they may be columns of one projection's rows). out may not overlap the inputs.
+ * max_q is at least every lq (later rows of a longer sequence are left as they are); max_k only guides
+ * how the work is cut. Offsets outside the arrays are cut to them. Rows of no sequence are not written.
+ * Keys behind a sequence's end or of a negative document may hold anything; other keys and values are
+ * finite, or a NaN can reach rows whose masks hide it. ws: workspace for calls with few rows over many
+ * keys, 16-byte aligned, laya_b200_attention_varlen_ws bytes for the same sizes (NULL or fewer bytes:
+ * the keys are cut into fewer ranges, with rounding differences); two calls in flight need two. */
+int laya_b200_attention_varlen(const void* q, long long ldq, const void* k, long long ldk, const void* v,
+                               long long ldv, void* out, long long ldo, float* lse, int type, const int* cu_q,
+                               const int* cu_k, int B, int rows_q, int rows_k, int max_q, int max_k, int Hq, int Hkv,
+                               int D, float scale, float softcap, const float* slopes, int left, int right,
+                               const int* prefix, const int* doc_q, const int* doc_k, void* ws, long long ws_bytes,
+                               void* stream, int sync);
+/* Workspace bytes for a call of these sizes on the current device (0: none), -1 no device, -2 refused. */
+long long laya_b200_attention_varlen_ws(int B, int rows_q, int max_q, int max_k, int Hq, int Hkv, int D);
+
 #ifdef __cplusplus
 }
 #endif

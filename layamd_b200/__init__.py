@@ -72,6 +72,9 @@ def load_lib(path: str = LIB_PATH) -> ctypes.CDLL:
         "laya_debug_bounds_build": (i, []),
         "laya_b200_norm": (i, [vp, i, ll, vp, i, ll, vp, i, ll, vp, vp, f, i, vp, i, ll, vp, i, i, vp, i]),
         "laya_b200_linear": (i, [vp, ll, vp, ll, i, vp, vp, vp, i, vp, ll, vp, i, ll, i, i, i, vp, i]),
+        "laya_b200_attention_varlen": (i, [vp, ll, vp, ll, vp, ll, vp, ll, vp, i, vp, vp, i, i, i, i, i, i, i, i, f, f,
+                                           vp, i, i, vp, vp, vp, vp, ll, vp, i]),
+        "laya_b200_attention_varlen_ws": (ll, [i, i, i, i, i, i, i]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -57,7 +57,7 @@ int begin(void* stream, int sync, std::initializer_list<const void*> arrays, Dev
   if (!g_dev[dev].ready) {
     if (cap != cudaStreamCaptureStatusNone) return -8;  // set-up allocates: not inside a capture
     if (cudaDeviceGetAttribute(&g_dev[dev].sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -4;
-    if (linear_prepare_device(&g_dev[dev].pairs) != cudaSuccess) return -4;
+    if (linear_prepare_device(&g_dev[dev].pairs) != cudaSuccess || varlen_prepare_device() != cudaSuccess) return -4;
     g_dev[dev].err = entry_error_word(dev);
     if (!g_dev[dev].err) return -4;
     g_dev[dev].ready = true;
@@ -137,4 +137,94 @@ extern "C" int laya_b200_linear(const void* A, long long lda, const void* W, lon
   const LinearArgs a{A, lda, W, ldw, a_scale, w_scale, bias, resid, ldr, out, ldo, ab_type, out_type, act, M, N, K, 0};
   return finish("linear", linear_launch(a, d.sms, d.pairs, d.err, static_cast<cudaStream_t>(stream)), stream, sync,
                 d.err);
+}
+
+namespace {
+// Bytes of the partial results of one key range.
+long long varlen_range_bytes(long long rows_q, int Hq, int D) { return rows_q * Hq * (D + 1LL) * 4; }
+
+bool varlen_sizes_ok(int B, int rows_q, int max_q, int max_k, int Hq, int Hkv, int D) {
+  return B >= 0 && B <= 65535 && rows_q >= 0 && rows_q <= kVarlenMaxRows && max_q >= 0 && max_q <= kVarlenMaxRows &&
+         max_k >= 0 && max_k <= kVarlenMaxRows && Hkv >= 1 && Hq >= Hkv && Hq <= 1024 && Hq % Hkv == 0 &&
+         (D == 64 || D == 128);
+}
+}  // namespace
+
+extern "C" long long laya_b200_attention_varlen_ws(int B, int rows_q, int max_q, int max_k, int Hq, int Hkv, int D) {
+  if (!varlen_sizes_ok(B, rows_q, max_q, max_k, Hq, Hkv, D)) return -2;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  const int splits = varlen_splits(B, max_q, max_k, Hq, Hkv, sms);
+  return splits > 1 ? splits * varlen_range_bytes(rows_q, Hq, D) : 0;
+}
+
+extern "C" int laya_b200_attention_varlen(const void* q, long long ldq, const void* k, long long ldk, const void* v,
+                                          long long ldv, void* out, long long ldo, float* lse, int type,
+                                          const int* cu_q, const int* cu_k, int B, int rows_q, int rows_k, int max_q,
+                                          int max_k, int Hq, int Hkv, int D, float scale, float softcap,
+                                          const float* slopes, int left, int right, const int* prefix,
+                                          const int* doc_q, const int* doc_k, void* ws, long long ws_bytes,
+                                          void* stream, int sync) {
+  if (!varlen_sizes_ok(B, rows_q, max_q, max_k, Hq, Hkv, D) || rows_k < 0 || rows_k > kVarlenMaxRows) return -2;
+  if (!is16(type) || !(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap)) return -2;
+  if (left < -1 || right < -1 || (doc_q == nullptr) != (doc_k == nullptr) || ws_bytes < 0) return -2;
+  if (B == 0 || rows_q == 0 || max_q == 0) return 0;
+  if (!q || !out || !cu_q || !cu_k || (rows_k > 0 && (!k || !v))) return -2;
+  const long long wq = (long long)Hq * D, wk = (long long)Hkv * D;
+  if (rows_q == 1) {  // one row has no stride of its own
+    if (ldq < wq) ldq = wq;
+    if (ldo < wq) ldo = wq;
+  }
+  if (rows_k <= 1) {
+    if (ldk < wk) ldk = wk;
+    if (ldv < wk) ldv = wk;
+  }
+  for (long long ld : {ldq - wq, ldk - wk, ldv - wk, ldo - wq})
+    if (ld < 0 || ld > kLinearMaxLd || ld % 8 != 0) return -2;  // rows start on 16 bytes
+  if (!is_aligned(q, 16) || !is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(out, 16) || !is_aligned(ws, 16) ||
+      !is_aligned(lse, 4) || !is_aligned(cu_q, 4) || !is_aligned(cu_k, 4) || !is_aligned(slopes, 4) ||
+      !is_aligned(prefix, 4) || !is_aligned(doc_q, 4) || !is_aligned(doc_k, 4))
+    return -2;
+  Device d;
+  if (int rc = begin(stream, sync, {q, k, v, out, lse, cu_q, cu_k, slopes, prefix, doc_q, doc_k, ws}, &d)) return rc;
+  VarlenArgs a;
+  a.q = q;
+  a.k = rows_k > 0 ? k : q;  // without keys nothing is read through the tensor maps, which need an address
+  a.v = rows_k > 0 ? v : q;
+  a.out = out;
+  a.ldq = ldq;
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.ldo = ldo;
+  a.lse = lse;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.B = B;
+  a.rows_q = rows_q;
+  a.rows_k = rows_k;
+  a.max_q = max_q < rows_q ? max_q : rows_q;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.D = D;
+  a.type = type;
+  a.scale = scale;
+  a.cap = softcap;
+  a.slopes = slopes;
+  a.left = left < 0 || left > kVarlenMaxRows ? kVarlenMaxRows : left;
+  a.right = right < 0 || right > kVarlenMaxRows ? kVarlenMaxRows : right;
+  a.prefix = prefix;
+  a.doc_q = doc_q;
+  a.doc_k = doc_k;
+  const long long range = varlen_range_bytes(rows_q, Hq, D);
+  const long long fit = ws ? ws_bytes / range : 0;
+  int splits = varlen_splits(B, a.max_q, max_k, Hq, Hkv, d.sms);
+  if (fit < splits) splits = fit > 1 ? static_cast<int>(fit) : 1;
+  a.splits = splits;
+  a.part_o = static_cast<float*>(ws);
+  a.part_l = a.part_o ? a.part_o + (long long)splits * rows_q * Hq * D : nullptr;
+  return finish("attention_varlen", varlen_launch(a, d.err, static_cast<cudaStream_t>(stream)), stream, sync, d.err);
 }

@@ -57,6 +57,34 @@ constexpr long long kLinearMaxLd = 1LL << 32;  // the tensor maps' strides stay 
 constexpr int kLinearFewRows = 16;  // most rows of the kernel for few rows
 cudaError_t linear_few_launch(const LinearArgs& a, int num_sms, cudaStream_t st);
 
+// Attention of packed sequences: s = scale q.k, capped by cap tanh(s / cap), minus slope |distance|,
+// then softmax over the keys that the window, prefix and document masks leave.
+struct VarlenArgs {
+  const void *q, *k, *v;
+  void* out;
+  long long ldq, ldk, ldv, ldo;
+  float* lse;          // [rows_q][Hq] or null
+  const int *cu_q, *cu_k;
+  int B, rows_q, rows_k, max_q;
+  int Hq, Hkv, D, type;
+  float scale, cap;    // cap 0: none
+  const float* slopes; // [Hq] or null
+  int left, right;     // kVarlenMaxRows: unbounded
+  const int* prefix;   // [B] or null
+  const int *doc_q, *doc_k;  // both or neither
+  int splits;          // key ranges per row; above 1 the partial results go to part_*
+  float* part_o;       // [splits][rows_q][Hq][D]
+  float* part_l;       // [splits][rows_q][Hq], log2 units
+};
+constexpr int kVarlenMaxRows = 1 << 29;  // positions and window edges stay in 32 bits
+constexpr int kVarlenMaxSplits = 32;
+cudaError_t varlen_prepare_device();
+// Key ranges that varlen_launch would use if the workspace allowed them.
+int varlen_splits(int B, int max_q, int max_k, int Hq, int Hkv, int num_sms);
+cudaError_t varlen_launch(const VarlenArgs& a, int* err, cudaStream_t st);
+bool varlen_few_rows(int max_q, int Hq, int Hkv);
+cudaError_t varlen_few_launch(const VarlenArgs& a, cudaStream_t st);
+
 // Tensor map of rows [rows][mid][cols] (strides in elements) loaded in 128-byte-wide boxes of box_rows
 // rows with the 128-byte swizzle; defined beside the engine's operand maps.
 bool make_rows_map(CUtensorMap* map, const void* base, int type, uint64_t cols, uint64_t mid, uint64_t rows,

@@ -39,3 +39,12 @@ def linear(A, W, out, a_scale=None, w_scale=None, bias=None, act=0, resid=None, 
                                        act, ptr(resid), ld(resid), ptr(out), code(out), ld(out),
                                        A.shape[0] if M is None else M, W.shape[0] if N is None else N,
                                        A.shape[1] if K is None else K, stream(), sync)
+
+
+def attention(q, k, v, out, lse, cu_q, cu_k, max_q, max_k, Hq, Hkv, D, scale=None, cap=0.0, slopes=None, left=-1,
+              right=-1, prefix=None, doc_q=None, doc_k=None, ws=None, sync=1):
+    return load_lib().laya_b200_attention_varlen(
+        ptr(q), ld(q), ptr(k), ld(k), ptr(v), ld(v), ptr(out), ld(out), ptr(lse), code(q), ptr(cu_q), ptr(cu_k),
+        cu_q.numel() - 1, q.shape[0], k.shape[0], max_q, max_k, Hq, Hkv, D, D ** -0.5 if scale is None else scale, cap,
+        ptr(slopes), left, right, ptr(prefix), ptr(doc_q), ptr(doc_k), ptr(ws), 0 if ws is None else ws.numel(),
+        stream(), sync)

@@ -68,3 +68,39 @@ def test_linear_accepts(L):
     dict(a_scale=A + 1), dict(w_scale=A + 3), dict(ab_type=E4M3, lda=72, ldw=72)])
 def test_linear_refuses(L, kw):
     assert L.laya_b200_linear(*linear_args(**kw)) == -2
+
+
+def attn_args(**kw):
+    a = dict(q=A, ldq=256, k=A, ldk=128, v=A, ldv=128, out=A, ldo=256, lse=A, type=BF16, cu_q=A, cu_k=A, B=2, rows_q=8,
+             rows_k=9, max_q=4, max_k=5, Hq=4, Hkv=2, D=64, scale=0.125, softcap=0.0, slopes=A, left=-1, right=0,
+             prefix=A, doc_q=A, doc_k=A, ws=None, ws_bytes=0, stream=None, sync=0)
+    a.update(kw)
+    return list(a.values())
+
+
+def test_attention_accepts(L):
+    f = L.laya_b200_attention_varlen
+    assert f(*attn_args()) == -1
+    assert f(*attn_args(lse=None, slopes=None, prefix=None, doc_q=None, doc_k=None)) == -1
+    assert f(*attn_args(rows_q=1, ldq=0, ldo=0, rows_k=1, ldk=0, ldv=0)) == -1
+    assert f(*attn_args(rows_k=0, k=None, v=None, ldk=0, ldv=0)) == -1
+    assert f(*attn_args(B=0)) == 0 and f(*attn_args(rows_q=0)) == 0 and f(*attn_args(max_q=0)) == 0
+    assert L.laya_b200_attention_varlen_ws(2, 8, 4, 5, 4, 2, 64) == -1
+
+
+@pytest.mark.parametrize("kw", [
+    dict(type=F32), dict(type=E4M3), dict(D=32), dict(D=96), dict(Hq=3), dict(Hkv=0), dict(Hq=2, Hkv=4),
+    dict(Hq=2048, Hkv=2), dict(B=-1), dict(B=65536), dict(rows_q=-1), dict(rows_k=-1), dict(rows_q=(1 << 29) + 1),
+    dict(max_q=-1), dict(max_k=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+    dict(scale=float("inf")), dict(softcap=-1.0), dict(softcap=float("nan")), dict(left=-2), dict(right=-2),
+    dict(doc_q=None), dict(doc_k=None), dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(cu_q=None),
+    dict(cu_k=None), dict(ldq=248), dict(ldq=260), dict(ldk=120), dict(ldv=129), dict(ldo=255), dict(ldo=1 << 33),
+    dict(q=A + 8), dict(k=A + 2), dict(v=A + 8), dict(out=A + 4), dict(lse=A + 2), dict(cu_q=A + 1), dict(ws=A + 8),
+    dict(ws_bytes=-1)])
+def test_attention_refuses(L, kw):
+    assert L.laya_b200_attention_varlen(*attn_args(**kw)) == -2
+
+
+def test_attention_workspace_refuses(L):
+    f = L.laya_b200_attention_varlen_ws
+    assert f(-1, 8, 4, 5, 4, 2, 64) == -2 and f(2, 8, 4, 5, 4, 3, 64) == -2 and f(2, 8, 4, 5, 4, 2, 80) == -2
