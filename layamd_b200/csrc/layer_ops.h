@@ -83,7 +83,8 @@ cudaError_t varlen_prepare_device();
 int varlen_splits(int B, int max_q, int max_k, int Hq, int Hkv, int num_sms);
 cudaError_t varlen_launch(const VarlenArgs& a, int* err, cudaStream_t st);
 bool varlen_few_rows(int max_q, int Hq, int Hkv);
-cudaError_t varlen_few_launch(const VarlenArgs& a, cudaStream_t st);
+cudaError_t varlen_few_prepare_device();
+cudaError_t varlen_few_launch(const VarlenArgs& a, int* err, cudaStream_t st);
 
 // Tensor map of rows [rows][mid][cols] (strides in elements) loaded in 128-byte-wide boxes of box_rows
 // rows with the 128-byte swizzle; defined beside the engine's operand maps.

@@ -1,49 +1,81 @@
 // Masked attention for few query rows (single tokens over long keys): every key and value is read once
 // and nearly nothing is computed, so the bound is HBM. A CTA takes up to 16 query rows that share a key
-// head (query heads of the group times query tokens) and a range of the keys; its 8 warps take 16 keys
-// each in turn.
-//
-// Operands go from memory straight into the registers of mma.sync m16n8k16. Its inner dimension may run
-// in any order, so in Q K^T each thread's 16 bytes of a key row take the places of the instruction's
-// K values; in P V the 8 output columns of one instruction are 8 dimensions that lie 8 apart, so that
-// a thread's 16 bytes of a value row serve 8 instructions. No shared memory in the loop: the next keys
-// load while the softmax and P V run, the next values while Q K^T does. The warps' partial rows (each
+// head (query heads of the group times query tokens) and a range of the keys. One warp streams 64-key
+// chunks of K and V by TMA into a ring of 6 stages (192 KB in flight per SM: two CTAs at head dim 64,
+// one at 128); the 8 others work in two groups that take the chunks in turn, 16 keys of a chunk per
+// warp, on mma.sync m16n8k16 with ldmatrix from the swizzled tiles. The warps' partial rows (each
 // with its own running maximum and sum) are joined through shared memory in warp order.
 //
-// Masked scores are replaced; values of keys that nobody may see are not read (zero), so that nothing
-// they hold reaches a row.
+// Single tokens of 24 sequences with up to 32,768 keys (1.8 GB of K and V): FEW_US us; operands loaded
+// straight into registers, with no more than 64 KB in flight per SM, took 461 us.
+//
+// Masked scores are replaced. Values of keys that nobody may see are set to zero in shared memory, so
+// that nothing they hold reaches a row.
+#include "kernels.h"
 #include "varlen.cuh"
 
 namespace laya {
 namespace {
 
-constexpr int kWarps = 8, kStep = 16 * kWarps;  // keys of one round of the warps
+constexpr int kWarps = 8, kKeys = 64, kStages = 6, kThreads = 32 * (kWarps + 1);
+constexpr uint32_t kAtom = kKeys * 128;  // 64 rows x 64 values
 
-__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                      uint32_t b1, bool bf) {
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool bf) {
   if (bf)
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16-byte piece `piece` of row `row` of a tile whose atoms are 64 columns (8 pieces) wide.
+__device__ __forceinline__ uint32_t tile_at(uint32_t tile, int row, int piece) {
+  return tile + (piece >> 3) * kAtom + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
 }
 
 template <int D>
 struct FewSmem {
-  float o[kWarps][16][D];
+  union {
+    struct {
+      uint8_t k[D / 64][kAtom], v[D / 64][kAtom];
+    } stage[kStages];
+    float o[kWarps][16][D];  // partial rows, once every chunk has been used
+  };
+  alignas(8) uint64_t full[kStages], empty[kStages];
+  int chunk[kStages];  // the chunk in a stage; -1: no more
   float m[kWarps][16], l[kWarps][16];
+  int abort;
 };
+template <int D>
+constexpr size_t smem_bytes() { return sizeof(FewSmem<D>) + 1024; }
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err, code));
+}
 
 template <int D, bool MOD>
-__global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) varlen_few_kernel(const VarlenArgs a) {
-  constexpr int kM = D / 32, kH = D / 64;
+__global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
+    varlen_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                      const VarlenArgs a, int* err) {
+  constexpr int kQ = D / 16;  // steps of 16 dimensions
   extern __shared__ uint8_t smem_raw[];
-  FewSmem<D>& S = *reinterpret_cast<FewSmem<D>*>(smem_raw);
+  FewSmem<D>& S = *reinterpret_cast<FewSmem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   pdl_trigger();
   pdl_wait();
   const int G = a.Hq / a.Hkv, row_tiles = (a.max_q * G + 15) / 16;
@@ -58,11 +90,28 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) varlen_few_kerne
   if (rt * 16 >= nrows) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const bool bf = a.type == DT_BF16;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_u32(&S.full[i]), 1);
+      mbar_init(smem_u32(&S.empty[i]), kWarps / 2);
+    }
+    S.abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  volatile int* abort = &S.abort;
+
+  // chunks that the masks can reach: the prefix's, then the window's
+  const int p_first = (rt * 16) / G + s.lk - s.lq, p_last = min(rt * 16 + 15, nrows - 1) / G + s.lk - s.lq;
+  const int wlo = max(0, p_first - a.left), whi = min(s.lk, p_last + a.right + 1);
+  const int end_a = (s.prefix + kKeys - 1) / kKeys;
+  const int beg_b = max(end_a, whi > wlo ? wlo / kKeys : 0);
+  const int end_b = whi > wlo ? (whi + kKeys - 1) / kKeys : 0;
+  const long long chunks = end_a + max(0, end_b - beg_b);
+  const int j0 = static_cast<int>(chunks * sp / a.splits), j1 = static_cast<int>(chunks * (sp + 1) / a.splits);
 
   // this thread's rows: g and g + 8 of the tile
   int pos[2], head[2], qdoc[2];
-  uint4 q[2][kM];
-  float slope[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int R = rt * 16 + g + 8 * r;
@@ -71,120 +120,131 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) varlen_few_kerne
     head[r] = hk * G + (on ? R - qi * G : 0);
     pos[r] = qi + s.lk - s.lq;
     qdoc[r] = a.doc_q ? (on ? a.doc_q[s.q0 + qi] : -1) : 0;
-    slope[r] = MOD && a.slopes ? a.slopes[head[r]] * kLog2e : 0.f;
-    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                      (long long)(s.q0 + qi) * a.ldq + head[r] * D);
-#pragma unroll
-    for (int m = 0; m < kM; ++m) q[r][m] = on ? __ldg(src + 4 * m + t) : make_uint4(0u, 0u, 0u, 0u);
   }
 
-  // rounds of 128 keys that the masks can reach: the prefix's, then the window's
-  const int p_first = (rt * 16) / G + s.lk - s.lq, p_last = min(rt * 16 + 15, nrows - 1) / G + s.lk - s.lq;
-  const int wlo = max(0, p_first - a.left), whi = min(s.lk, p_last + a.right + 1);
-  const int end_a = (s.prefix + kStep - 1) / kStep;
-  const int beg_b = max(end_a, whi > wlo ? wlo / kStep : 0);
-  const int end_b = whi > wlo ? (whi + kStep - 1) / kStep : 0;
-  const long long rounds = end_a + max(0, end_b - beg_b);
-  const int j0 = static_cast<int>(rounds * sp / a.splits), j1 = static_cast<int>(rounds * (sp + 1) / a.splits);
-  auto key_of = [&](int j) { return (j < end_a ? j : j - end_a + beg_b) * kStep + warp * 16; };
-
-  int doc_lo = 0, doc_hi = 0;
-  if (a.doc_k) {
-    const int lo0 = qdoc[0] < 0 ? 0x7fffffff : qdoc[0], lo1 = qdoc[1] < 0 ? 0x7fffffff : qdoc[1];
-    doc_lo = __reduce_min_sync(0xffffffffu, min(lo0, lo1));
-    doc_hi = __reduce_max_sync(0xffffffffu, max(qdoc[0], qdoc[1]));
+  if (warp == kWarps) {
+    // ---------------- TMA producer
+    int doc_lo = 0, doc_hi = 0;
+    if (a.doc_k) {
+      const int lo0 = qdoc[0] < 0 ? 0x7fffffff : qdoc[0], lo1 = qdoc[1] < 0 ? 0x7fffffff : qdoc[1];
+      doc_lo = __reduce_min_sync(0xffffffffu, min(lo0, lo1));
+      doc_hi = __reduce_max_sync(0xffffffffu, max(qdoc[0], qdoc[1]));
+    }
+    int n = 0;
+    bool ok = true;
+    auto stage_free = [&]() {
+      const int st = n % kStages;
+      return n < kStages ||
+             __all_sync(0xffffffffu, mbar_wait(smem_u32(&S.empty[st]), ((n / kStages) - 1) & 1, abort, err, kErrAttnLoad));
+    };
+    for (int j = j0; ok && j < j1; ++j) {
+      const int c = j < end_a ? j : j - end_a + beg_b;
+      if (a.doc_k) {  // a chunk without a key of the rows' documents is not read
+        const int k = c * kKeys + lane;
+        const int x = k < s.lk ? __ldg(a.doc_k + s.k0 + k) : -1, y = k + 32 < s.lk ? __ldg(a.doc_k + s.k0 + k + 32) : -1;
+        const bool hit = (x >= 0 && x >= doc_lo && x <= doc_hi) || (y >= 0 && y >= doc_lo && y <= doc_hi);
+        if (!__any_sync(0xffffffffu, hit)) continue;
+      }
+      if (!stage_free()) { ok = false; break; }
+      if (lane == 0) {
+        const int st = n % kStages;
+        const uint32_t fb = smem_u32(&S.full[st]);
+        S.chunk[st] = c;
+        mbar_expect_tx(fb, 2 * (D / 64) * kAtom);
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d) {
+          tma_load_3d(smem_u32(S.stage[st].k[d]), &tk, d * 64, hk, s.k0 + c * kKeys, fb);
+          tma_load_3d(smem_u32(S.stage[st].v[d]), &tv, d * 64, hk, s.k0 + c * kKeys, fb);
+        }
+      }
+      __syncwarp();
+      ++n;
+    }
+    const int loads = n;
+    for (int i = 0; ok && i < 2; ++i) {  // the end, once for each group
+      if (!stage_free()) { ok = false; break; }
+      if (lane == 0) {
+        S.chunk[n % kStages] = -1;
+        mbar_arrive(smem_u32(&S.full[n % kStages]));
+      }
+      __syncwarp();
+      ++n;
+    }
+    if (!ok && lane == 0) {  // the loads in flight land before the CTA can exit
+      const long long t0 = clock64();
+      for (int st = 0; st < kStages; ++st) {
+        const int issued = (loads - st + kStages - 1) / kStages;
+        if (issued <= 0) continue;
+        while (!mbar_try(smem_u32(&S.full[st]), (issued - 1) & 1))
+          if (clock64() - t0 > kWaitBudgetCycles) { atomicCAS(err, 0, kErrGemmDrain); break; }
+      }
+    }
+    __syncwarp();
+    __syncthreads();
+    return;
   }
-  // The rounds of the 32 from `base` on that hold a key of a document in [doc_lo, doc_hi] for this warp.
-  auto active = [&](int base) -> uint32_t {
-    const int j = base + lane;
-    bool hit = j < j1;
-    if (a.doc_k && hit) {
-      const int kb = key_of(j);
-      hit = false;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int id = kb + i < s.lk ? __ldg(a.doc_k + s.k0 + kb + i) : -1;
-        hit = hit || (id >= 0 && id >= doc_lo && id <= doc_hi);
-      }
-    }
-    return __ballot_sync(0xffffffffu, hit);
-  };
-  int base = j0;
-  uint32_t todo = active(base);
-  auto next_round = [&]() -> int {  // -1 at the end
-    while (todo == 0) {
-      base += 32;
-      if (base >= j1) return -1;
-      todo = active(base);
-    }
-    const int i = __ffs(todo) - 1;
-    todo &= todo - 1;
-    return base + i;
-  };
 
-  const char* kp = static_cast<const char*>(a.k) + ((long long)s.k0 * a.ldk + hk * D) * 2;
-  const char* vp = static_cast<const char*>(a.v) + ((long long)s.k0 * a.ldv + hk * D) * 2;
-  uint4 kr[2][kM], vr[4][kH];
-  int kid = 0, kid_next = 0;  // document of key kb + lane % 16
-  auto load_k = [&](int kb) {
-    if (a.doc_k) kid_next = kb + (lane & 15) < s.lk ? __ldg(a.doc_k + s.k0 + kb + (lane & 15)) : -1;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int key = kb + 8 * i + g;
-      const uint4* src = reinterpret_cast<const uint4*>(kp + (long long)key * a.ldk * 2);
-#pragma unroll
-      for (int m = 0; m < kM; ++m) kr[i][m] = key < s.lk ? __ldcs(src + 4 * m + t) : make_uint4(0u, 0u, 0u, 0u);
-    }
-  };
-  auto load_v = [&](int kb, int id) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int off = 2 * t + (r & 1) + 8 * (r >> 1), key = kb + off;
-      bool on = key < s.lk;
-      if (a.doc_k) {  // the whole warp
-        const int doc = __shfl_sync(0xffffffffu, id, off);
-        on = on && doc >= 0;
-      }
-      const uint4* src = reinterpret_cast<const uint4*>(vp + (long long)key * a.ldv * 2);
-#pragma unroll
-      for (int h = 0; h < kH; ++h) vr[r][h] = on ? __ldcs(src + 8 * h + g) : make_uint4(0u, 0u, 0u, 0u);
-    }
-  };
-
+  // ---------------- consumers: warp w takes keys 16 (w % 4) .. of its group's chunks
+  const int group = warp >> 2, key0 = 16 * (warp & 3);
+  uint32_t q[kQ][4];
+  float slope[2];
   const float cs = a.scale * kLog2e;
   const float cap_in = MOD && a.cap > 0.f ? a.scale / a.cap : 0.f, cap_out = a.cap * kLog2e;
-  float o[kH][8][4];
 #pragma unroll
-  for (int h = 0; h < kH; ++h)
+  for (int r = 0; r < 2; ++r) {
+    slope[r] = MOD && a.slopes ? a.slopes[head[r]] * kLog2e : 0.f;
+    const bool on = rt * 16 + g + 8 * r < nrows;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(
+        static_cast<const uint16_t*>(a.q) + (long long)(s.q0 + pos[r] - s.lk + s.lq) * a.ldq + head[r] * D);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[h][j][e] = 0.f;
-  float mr[2] = {-INFINITY, -INFINITY}, lr[2] = {0.f, 0.f};
-
-  int j = j0 < j1 ? next_round() : -1;
-  if (j >= 0) {
-    load_k(key_of(j));
-    kid = kid_next;
-    load_v(key_of(j), kid);
+    for (int i = 0; i < kQ; ++i) {
+      q[i][r] = on ? __ldg(src + 8 * i + t) : 0u;
+      q[i][r + 2] = on ? __ldg(src + 8 * i + 4 + t) : 0u;
+    }
   }
-  while (j >= 0) {
-    const int kb = key_of(j);
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  float mr[2] = {-INFINITY, -INFINITY}, lr[2] = {0.f, 0.f};
+  // ldmatrix rows of this lane: K matrices (keys 0-7, 8-15) x (dims 0-7, 8-15), V ones transposed
+  const int k_row = key0 + (lane & 7) + ((lane >> 4) << 3), k_piece = (lane >> 3) & 1;
+  const int v_row = key0 + (lane & 15), v_piece = lane >> 4;
+
+  for (int n = group;; n += 2) {
+    const int st = n % kStages;
+    if (!warp_wait(smem_u32(&S.full[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) break;
+    const int c = *static_cast<volatile int*>(&S.chunk[st]);
+    if (c < 0) break;
+    const int kb = c * kKeys + key0;
+    int kid = 0;  // document of key kb + lane % 16
+    if (a.doc_k) kid = kb + (lane & 15) < s.lk ? __ldg(a.doc_k + s.k0 + kb + (lane & 15)) : -1;
+    const uint32_t kt = smem_u32(S.stage[st].k[0]), vt = smem_u32(S.stage[st].v[0]);
     float x[2][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
 #pragma unroll
-      for (int m = 0; m < kM; ++m) {
-        const uint4 w = kr[i][m];
-        mma16(x[i], q[0][m].x, q[1][m].x, q[0][m].y, q[1][m].y, w.x, w.y, bf);
-        mma16(x[i], q[0][m].z, q[1][m].z, q[0][m].w, q[1][m].w, w.z, w.w, bf);
-      }
+    for (int i = 0; i < kQ; ++i) {
+      uint32_t b[4];
+      ldmatrix4(b, tile_at(kt, k_row, 2 * i + k_piece));
+      mma16(x[0], q[i], b[0], b[1], bf);
+      mma16(x[1], q[i], b[2], b[3], bf);
     }
-    const int j_next = next_round();
-    if (j_next >= 0) load_k(key_of(j_next));
-
+    // keys that nobody may see: their values are zero from here on
+    const bool dead = kb + (lane & 15) >= s.lk || (a.doc_k && kid < 0);
+    if (__any_sync(0xffffffffu, dead)) {
+      if (dead) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)  // lanes l and l + 16 share a row
+          *reinterpret_cast<uint4*>(S.stage[st].v[0] + (tile_at(vt, key0 + (lane & 15), 2 * i + (lane >> 4)) - vt)) =
+              make_uint4(0u, 0u, 0u, 0u);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage is loaded again
+      __syncwarp();
+    }
     // x[i][2 r + e]: row g + 8 r, key kb + 8 i + 2 t + e
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -228,15 +288,13 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) varlen_few_kerne
         mr[r] = m_new;
         lr[r] *= alpha;
 #pragma unroll
-        for (int h = 0; h < kH; ++h)
-#pragma unroll
-          for (int jj = 0; jj < 8; ++jj) {
-            o[h][jj][2 * r] *= alpha;
-            o[h][jj][2 * r + 1] *= alpha;
-          }
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][2 * r] *= alpha;
+          o[i][2 * r + 1] *= alpha;
+        }
       }
     }
-    uint32_t pa[2][2];  // [key group][row]
+    uint32_t pa[4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float sub = mr[r] == -INFINITY ? 0.f : mr[r];
@@ -244,48 +302,37 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) varlen_few_kerne
       for (int i = 0; i < 2; ++i) {
         const float p0 = exp2_fast(x[i][2 * r] - sub), p1 = exp2_fast(x[i][2 * r + 1] - sub);
         lr[r] += p0 + p1;
-        pa[i][r] = pack_pair(p0, p1, a.type);
+        pa[2 * i + r] = pack_pair(p0, p1, a.type);
       }
     }
-    // column n of instruction (h, jj) is dimension 64 h + 8 n + jj
 #pragma unroll
-    for (int h = 0; h < kH; ++h) {
-      const uint32_t v0[4] = {vr[0][h].x, vr[0][h].y, vr[0][h].z, vr[0][h].w};
-      const uint32_t v1[4] = {vr[1][h].x, vr[1][h].y, vr[1][h].z, vr[1][h].w};
-      const uint32_t v2[4] = {vr[2][h].x, vr[2][h].y, vr[2][h].z, vr[2][h].w};
-      const uint32_t v3[4] = {vr[3][h].x, vr[3][h].y, vr[3][h].z, vr[3][h].w};
-#pragma unroll
-      for (int jj = 0; jj < 8; ++jj) {
-        const uint32_t sel = jj & 1 ? 0x7632 : 0x5410;
-        mma16(o[h][jj], pa[0][0], pa[0][1], pa[1][0], pa[1][1], __byte_perm(v0[jj / 2], v1[jj / 2], sel),
-              __byte_perm(v2[jj / 2], v3[jj / 2], sel), bf);
-      }
+    for (int i = 0; i < D / 16; ++i) {
+      uint32_t b[4];
+      ldmatrix4_t(b, tile_at(vt, v_row, 2 * i + v_piece));
+      mma16(o[2 * i], pa, b[0], b[1], bf);
+      mma16(o[2 * i + 1], pa, b[2], b[3], bf);
     }
-    j = j_next;
-    kid = kid_next;
-    if (j >= 0) load_v(key_of(j), kid);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&S.empty[st]));
   }
 
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     lr[r] += __shfl_xor_sync(0xffffffffu, lr[r], 1);
     lr[r] += __shfl_xor_sync(0xffffffffu, lr[r], 2);
+  }
+  __syncthreads();  // every chunk has been used: the stages take the partial rows
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
     if (t == 0) {
       S.m[warp][g + 8 * r] = mr[r];
       S.l[warp][g + 8 * r] = lr[r];
     }
 #pragma unroll
-    for (int h = 0; h < kH; ++h) {
-      float4* dst = reinterpret_cast<float4*>(&S.o[warp][g + 8 * r][64 * h + 16 * t]);
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          dst[2 * e + c] = make_float4(o[h][4 * c][2 * r + e], o[h][4 * c + 1][2 * r + e], o[h][4 * c + 2][2 * r + e],
-                                       o[h][4 * c + 3][2 * r + e]);
-    }
+    for (int i = 0; i < D / 8; ++i)
+      *reinterpret_cast<float2*>(&S.o[warp][g + 8 * r][8 * i + 2 * t]) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
   }
-  __syncthreads();
+  asm volatile("bar.sync 1, 256;" ::: "memory");  // the consumers
   // 16 threads a row join the warps' partial rows
   const int row = threadIdx.x >> 4, c0 = (threadIdx.x & 15) * (D / 16);
   const int R = rt * 16 + row;
@@ -321,26 +368,43 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) varlen_few_kerne
 }
 
 template <int D>
-cudaError_t launch(const VarlenArgs& a, cudaStream_t st) {
+cudaError_t launch(const VarlenArgs& a, int* err, cudaStream_t st) {
+  CUtensorMap tk, tv;
+  auto map = [&](CUtensorMap* m, const void* base, long long ld) {
+    return make_rows_map(m, base, a.type, D, static_cast<uint64_t>(a.Hkv), static_cast<uint64_t>(a.rows_k > 0 ? a.rows_k : 1), D,
+                         static_cast<uint64_t>(ld), kKeys);
+  };
+  if (!map(&tk, a.k, a.ldk) || !map(&tv, a.v, a.ldv)) return cudaErrorInvalidValue;
   const int G = a.Hq / a.Hkv;
   const long long grid = (long long)((a.max_q * G + 15) / 16) * a.splits * a.Hkv * a.B;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
   const dim3 g(static_cast<unsigned>(grid));
-  auto go = [&](auto kernel) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(FewSmem<D>)));
-    return e != cudaSuccess ? e : launch_pdl(kernel, g, dim3(32 * kWarps), sizeof(FewSmem<D>), st, a);
-  };
-  return a.cap > 0.f || a.slopes ? go(varlen_few_kernel<D, true>) : go(varlen_few_kernel<D, false>);
+  return a.cap > 0.f || a.slopes
+             ? launch_pdl(varlen_few_kernel<D, true>, g, dim3(kThreads), smem_bytes<D>(), st, tk, tv, a, err)
+             : launch_pdl(varlen_few_kernel<D, false>, g, dim3(kThreads), smem_bytes<D>(), st, tk, tv, a, err);
+}
+
+template <int D>
+cudaError_t prepare() {
+  const int bytes = static_cast<int>(smem_bytes<D>());
+  const cudaError_t e =
+      cudaFuncSetAttribute(varlen_few_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(varlen_few_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 }  // namespace
 
+cudaError_t varlen_few_prepare_device() {
+  const cudaError_t e = prepare<64>();
+  return e != cudaSuccess ? e : prepare<128>();
+}
+
 // Rows that share a key head: up to four tiles of 16 are cheaper here than one of 128 per head.
 bool varlen_few_rows(int max_q, int Hq, int Hkv) { return (long long)max_q * (Hq / Hkv) <= 64; }
 
-cudaError_t varlen_few_launch(const VarlenArgs& a, cudaStream_t st) {
-  return a.D == 64 ? launch<64>(a, st) : launch<128>(a, st);
+cudaError_t varlen_few_launch(const VarlenArgs& a, int* err, cudaStream_t st) {
+  return a.D == 64 ? launch<64>(a, err, st) : launch<128>(a, err, st);
 }
 
 }  // namespace laya

@@ -130,6 +130,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   // row of this thread (softmax warps): TMEM lanes 32 * (warp % 4) .. belong to warp
   const int qw = warp & 3, row = qw * 32 + lane;
   int qdoc = 0;
+  if (a.doc_q) {
+    for (int i = threadIdx.x; i < kDocWords; i += kThreads) S.docs[i] = 0u;
+  }
   if (a.doc_q && warp >= 2) {
     qdoc = row < rows ? a.doc_q[s.q0 + t0 + row] : -1;
     const int lo = __reduce_min_sync(0xffffffffu, qdoc < 0 ? 0x7fffffff : qdoc);
@@ -154,16 +157,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int lo = min(min(S.doc_lo[0], S.doc_lo[1]), min(S.doc_lo[2], S.doc_lo[3]));
     const int hi = max(max(S.doc_hi[0], S.doc_hi[1]), max(S.doc_hi[2], S.doc_hi[3]));
     const int* ids = a.doc_k + s.k0;
-    for (int w = (ch.lo >> 5) + warp; w < kDocWords && w * 32 < ch.hi; w += kThreads / 32) {
-      uint32_t word = 0;
-#pragma unroll 8
-      for (int i = 0; i < 32; ++i) {
-        const int k = (w * 32 + i) * kKeys + lane;
-        const int x = k < s.lk ? ids[k] : -1, y = k + 32 < s.lk ? ids[k + 32] : -1;
-        const bool hit = (x >= lo && x <= hi && x >= 0) || (y >= lo && y <= hi && y >= 0);
-        if (__any_sync(0xffffffffu, hit)) word |= 1u << i;
-      }
-      if (lane == 0) S.docs[w] = word;
+    const int end = min(ch.hi, kDocWords * 32);
+#pragma unroll 4
+    for (int c = ch.lo + warp; c < end; c += kThreads / 32) {
+      const int k = c * kKeys + lane;
+      const int x = k < s.lk ? ids[k] : -1, y = k + 32 < s.lk ? ids[k + 32] : -1;
+      const bool hit = (x >= lo && x <= hi && x >= 0) || (y >= lo && y <= hi && y >= 0);
+      if (__any_sync(0xffffffffu, hit) && lane == 0) atomicOr(&S.docs[c >> 5], 1u << (c & 31));
     }
   }
   tc_fence_before();
@@ -257,11 +257,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
   } else {
-    // ---------------- softmax: scores in log2 units
+    // ---------------- softmax: scores stay in units of q.k until the exponential scales them
     const uint32_t tl = tmem + (static_cast<uint32_t>(qw * 32) << 16);
     const float cs = a.scale * kLog2e;
-    const float cap_in = a.cap > 0.f ? a.scale / a.cap : 0.f, cap_out = a.cap * kLog2e;
-    const float slope = MOD && a.slopes ? a.slopes[h] * kLog2e : 0.f;
+    const float cap_in = a.cap > 0.f ? a.scale / a.cap : 0.f, cap_out = a.cap / a.scale;
+    const float slope = MOD && a.slopes ? a.slopes[h] / a.scale : 0.f;
     const int p = p0 + row;             // this row's key position
     const int pw = p0 + qw * 32;        // the warp's first and last
     const int pz = pw + 31;
@@ -315,15 +315,22 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int i = 0; i < 64; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
           if (__all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
+            // the polynomial in the squared score, two lanes an instruction
+            const float z1 = cap_in * cap_in, k1 = -z1 / 3.f, k2 = z1 * z1 * (2.f / 15.f),
+                        k3 = z1 * z1 * z1 * (-17.f / 315.f);
+            const float2 c1 = make_float2(k1, k1), c2 = make_float2(k2, k2), c3 = make_float2(k3, k3),
+                         one = make_float2(1.f, 1.f);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) x[i] = cap_out * tanh_small(x[i] * cap_in);
+            for (int i = 0; i < 64; i += 2) {
+              const float2 v = make_float2(x[i], x[i + 1]), z = __fmul2_rn(v, v);
+              const float2 r = __fmul2_rn(v, __ffma2_rn(z, __ffma2_rn(z, __ffma2_rn(z, c3, c2), c1), one));
+              x[i] = r.x;
+              x[i + 1] = r.y;
+            }
           } else {
 #pragma unroll
             for (int i = 0; i < 64; ++i) x[i] = cap_out * tanh_any(x[i] * cap_in);
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) x[i] *= cs;
         }
         if (a.slopes) {
           const float away = static_cast<float>(p - k0);
@@ -352,8 +359,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int i = 0; i < 32; i += 2) mq[(i >> 1) & 3] = max3(mq[(i >> 1) & 3], x[32 * g + i], x[32 * g + i + 1]);
         }
       }
-      const float mul = MOD ? 1.f : cs;
-      const float mx = max3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * mul;
+      const float mx = max3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * cs;
       const float m_new = fmaxf(m_used, mx);
       const bool resc = m_new > m_used + 8.f;
       const bool resc_o = resc && m_used != -INFINITY;  // O is exactly 0 before a row's first visible key
@@ -364,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         m_used = m_new;
       }
       const float msub = m_used == -INFINITY ? 0.f : m_used;
-      const float2 mul2 = make_float2(mul, mul), nm2 = make_float2(-msub, -msub);
+      const float2 mul2 = make_float2(cs, cs), nm2 = make_float2(-msub, -msub);
       uint32_t pk[32];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
@@ -518,8 +524,8 @@ cudaError_t launch(const VarlenArgs& a, int* err, cudaStream_t st) {
     return make_rows_map(m, base, a.type, D, static_cast<uint64_t>(heads), static_cast<uint64_t>(rows), D,
                          static_cast<uint64_t>(ld), static_cast<uint32_t>(box));
   };
-  if (!map(&tq, a.q, a.Hq, a.rows_q, a.ldq, kRows) || !map(&tk, a.k, a.Hkv, a.rows_k, a.ldk, kKeys) ||
-      !map(&tv, a.v, a.Hkv, a.rows_k, a.ldv, kKeys))
+  if (!map(&tq, a.q, a.Hq, a.rows_q, a.ldq, kRows) || !map(&tk, a.k, a.Hkv, std::max(1, a.rows_k), a.ldk, kKeys) ||
+      !map(&tv, a.v, a.Hkv, std::max(1, a.rows_k), a.ldv, kKeys))
     return cudaErrorInvalidValue;
   const long long grid = (long long)((a.max_q + kRows - 1) / kRows) * a.B * a.Hq * a.splits;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
@@ -541,8 +547,9 @@ cudaError_t prepare() {
 }  // namespace
 
 cudaError_t varlen_prepare_device() {
-  const cudaError_t e = prepare<64>();
-  return e != cudaSuccess ? e : prepare<128>();
+  for (cudaError_t e : {prepare<64>(), prepare<128>(), varlen_few_prepare_device()})
+    if (e != cudaSuccess) return e;
+  return cudaSuccess;
 }
 
 int varlen_splits(int B, int max_q, int max_k, int Hq, int Hkv, int num_sms) {
@@ -551,12 +558,12 @@ int varlen_splits(int B, int max_q, int max_k, int Hq, int Hkv, int num_sms) {
   const long long units = few ? (long long)B * Hkv * ((max_q * (Hq / Hkv) + 15) / 16)
                               : (long long)B * Hq * ((max_q + kRows - 1) / kRows);
   const long long most = std::max<long long>(1, max_k / (few ? 512 : 4 * kKeys));
-  const long long want = units > 0 ? 2LL * num_sms / units : 1;
+  const long long want = units > 0 ? (few ? 8LL : 2LL) * num_sms / units : 1;
   return static_cast<int>(std::max<long long>(1, std::min<long long>({want, most, kVarlenMaxSplits})));
 }
 
 cudaError_t varlen_launch(const VarlenArgs& a, int* err, cudaStream_t st) {
-  cudaError_t e = varlen_few_rows(a.max_q, a.Hq, a.Hkv) ? varlen_few_launch(a, st)
+  cudaError_t e = varlen_few_rows(a.max_q, a.Hq, a.Hkv) ? varlen_few_launch(a, err, st)
                   : a.D == 64                           ? launch<64>(a, err, st)
                                                         : launch<128>(a, err, st);
   if (e != cudaSuccess || a.splits == 1) return e;

@@ -301,6 +301,11 @@ def test_nothing_to_do():
         assert attention(q, none, none, out, None, c, offsets([0]), mq, 0, 1, 1, 64) == 0
     torch.cuda.synchronize()
     assert bool((out == 0).all())
+    many = torch.randn(200, 64, device="cuda").to(BF)
+    out = torch.full_like(many, 7.0)
+    assert attention(many, none, none, out, None, offsets([200]), offsets([0]), 200, 0, 1, 1, 64) == 0
+    torch.cuda.synchronize()
+    assert bool((out == 0).all())
 
 
 @pytest.mark.parametrize("lq,lk", [([300, 77], None), ([1, 1], [5000, 3000])])
