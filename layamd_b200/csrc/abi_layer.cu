@@ -226,5 +226,5 @@ extern "C" int laya_b200_attention_varlen(const void* q, long long ldq, const vo
   a.splits = splits;
   a.part_o = static_cast<float*>(ws);
   a.part_l = a.part_o ? a.part_o + (long long)splits * rows_q * Hq * D : nullptr;
-  return finish("attention_varlen", varlen_launch(a, d.err, static_cast<cudaStream_t>(stream)), stream, sync, d.err);
+  return finish("attention_varlen", varlen_launch(a, d.sms, d.err, static_cast<cudaStream_t>(stream)), stream, sync, d.err);
 }

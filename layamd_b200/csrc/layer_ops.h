@@ -81,7 +81,7 @@ constexpr int kVarlenMaxSplits = 32;
 cudaError_t varlen_prepare_device();
 // Key ranges that varlen_launch would use if the workspace allowed them.
 int varlen_splits(int B, int max_q, int max_k, int Hq, int Hkv, int num_sms);
-cudaError_t varlen_launch(const VarlenArgs& a, int* err, cudaStream_t st);
+cudaError_t varlen_launch(const VarlenArgs& a, int num_sms, int* err, cudaStream_t st);
 bool varlen_few_rows(int max_q, int Hq, int Hkv);
 cudaError_t varlen_few_prepare_device();
 cudaError_t varlen_few_launch(const VarlenArgs& a, int* err, cudaStream_t st);

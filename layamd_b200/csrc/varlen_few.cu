@@ -82,10 +82,10 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
   int u = static_cast<int>(blockIdx.x);
   const int rt = u % row_tiles;
   u /= row_tiles;
+  const int hk = u % a.Hkv;  // heads next to one another in memory run together
+  u /= a.Hkv;
   const int sp = u % a.splits;
-  u /= a.splits;
-  const int hk = u % a.Hkv;
-  const Sequence s = sequence(a, u / a.Hkv);
+  const Sequence s = sequence(a, u / a.splits);
   const int nrows = min(s.lq, a.max_q) * G;  // (token, head of the group) rows of this key head
   if (rt * 16 >= nrows) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
   }
 
   // ---------------- consumers: warp w takes keys 16 (w % 4) .. of its group's chunks
+  const bool two = nrows - rt * 16 > 8;  // rows 8 .. 15 of the tile hold anything
   const int group = warp >> 2, key0 = 16 * (warp & 3);
   uint32_t q[kQ][4];
   float slope[2];
@@ -246,34 +247,47 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       __syncwarp();
     }
     // x[i][2 r + e]: row g + 8 r, key kb + 8 i + 2 t + e
+    const bool full = !a.doc_k && kb + 16 <= s.lk &&
+                      ((kb >= p_last - a.left && kb + 15 <= p_first + a.right) || kb + 16 <= s.prefix);
+    bool small = false;
+    if (MOD && a.cap > 0.f) {
+      float big = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = e >> 1, off = 8 * i + 2 * t + (e & 1), key = kb + off;
-        float v = x[i][e];
-        if constexpr (MOD) {
-          if (a.cap > 0.f) {
-            const float in = v * cap_in;
-            v = cap_out * (fabsf(in) < kTanhSmall ? tanh_small(in) : tanh_any(in));
-          } else {
-            v *= cs;
-          }
-          v = fmaf(-slope[r], fabsf(static_cast<float>(pos[r] - key)), v);
-        } else {
-          v *= cs;
-        }
-        bool see = key < s.lk && ((key >= pos[r] - a.left && key <= pos[r] + a.right) || key < s.prefix);
-        if (a.doc_k) {
-          const int id = __shfl_sync(0xffffffffu, kid, off);
-          see = see && id >= 0 && id == qdoc[r];
-        }
-        x[i][e] = see ? v : -INFINITY;
-      }
-    float top[2];
+        for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[i][e]));
+      small = __all_sync(0xffffffffu, big * cap_in < kTanhSmall);
+    }
+    float top[2] = {-INFINITY, -INFINITY};
     bool up = false;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
+      if (r == 1 && !two) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 2 * r; e < 2 * r + 2; ++e) {
+          const int off = 8 * i + 2 * t + (e & 1), key = kb + off;
+          float v = x[i][e];
+          if constexpr (MOD) {
+            if (a.cap > 0.f)
+              v = small ? cap_out * tanh_small(v * cap_in) : cap_out * tanh_any(v * cap_in);
+            else
+              v *= cs;
+            if (a.slopes) v = fmaf(-slope[r], fabsf(static_cast<float>(pos[r] - key)), v);
+          } else {
+            v *= cs;
+          }
+          if (!full) {
+            bool see = key < s.lk && ((key >= pos[r] - a.left && key <= pos[r] + a.right) || key < s.prefix);
+            if (a.doc_k) {
+              const int id = __shfl_sync(0xffffffffu, kid, off);
+              see = see && id >= 0 && id == qdoc[r];
+            }
+            if (!see) v = -INFINITY;
+          }
+          x[i][e] = v;
+        }
       top[r] = fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]));
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
@@ -294,9 +308,10 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
         }
       }
     }
-    uint32_t pa[4];
+    uint32_t pa[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
+      if (r == 1 && !two) break;
       const float sub = mr[r] == -INFINITY ? 0.f : mr[r];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {

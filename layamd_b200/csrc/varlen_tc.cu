@@ -1,25 +1,28 @@
 // Masked attention of packed sequences on the 5th-generation tensor cores (TMA + tcgen05 + TMEM), head
-// dim 64 or 128, shared key heads: each CTA takes 128 query rows of one sequence and head and walks the
-// 64-key chunks that its masks can reach, with the running maximum and sum of the softmax.
+// dim 64 or 128, shared key heads. A work unit is 128 query rows of one sequence and head (and, with
+// splits > 1, one range of the keys); it walks the 64-key chunks that its masks can reach, with the
+// running maximum and sum of the softmax.
 //
-// Two CTAs per SM (192 threads, 256 TMEM columns each), so that one CTA's products run under the
-// other's exponentials and prologue:
-//   warp 0      TMA producer: Q once, then K and V chunks into two rings (4 stages at head dim 64, 2 at
-//               128), a K stage released when its scores are formed, a V stage when its product is
+// Persistent, two CTAs per SM (192 threads, 256 TMEM columns each), so that one CTA's products run
+// under the other's exponentials; units go round the CTAs, longest tiles first (causal rows near the
+// end), heads fastest, so that the units in flight share keys in L2. Within a CTA the units run through
+// one pipeline across their borders:
+//   warp 0      TMA producer: finds a unit's sequence and its chunks, publishes them through a ring in
+//               shared memory, loads Q (2 slots at head dim 64) and the K and V chunks into two rings
+//               (4 stages at head dim 64, 2 at 128), running ahead into the next units; a K stage is
+//               free when its scores are formed, a V stage when its product is
 //   warp 1      MMA issuer: S = Q K^T (128 x 64 fp32, one TMEM buffer, reformed as soon as the softmax
 //               warps have copied it) and O += P V (P from TMEM, V MN-major from its TMA tile)
-//   warps 2..5  softmax, one query row per thread
+//   warps 2..5  softmax, one query row per thread; a unit's O / l is written during the next unit's
+//               first chunk (after it at head dim 64, where O has two buffers)
 // Chunks are skipped whole where the window, the prefix or the documents leave nothing; a document's
-// chunks are found once per CTA from the key ids, 32 chunks a word. Inside a chunk, groups of 32 keys
-// that every row of a warp sees skip the masking. The reference maximum is raised only when it grows by
-// more than 2^8, so O is rarely rescaled.
+// chunks are found once per unit from the key ids. Inside a chunk, groups of 32 keys that every row of
+// a warp sees skip the masking. The reference maximum is raised only when it grows by more than 2^8, so
+// O is rarely rescaled.
 //
 // A masked score is replaced, so K may hold anything there. Keys that nobody may see (behind the
 // sequence's end, or of document -1) meet P = 0 in the product, and 0 * NaN would spoil the row: their
 // V rows are set to zero in shared memory before the product is issued.
-//
-// The longest tiles come first (causal rows near the end), heads fastest, so that the CTAs in flight
-// share keys in L2. With splits > 1 a CTA takes one range of the chunks and leaves fp32 partial rows.
 #include <algorithm>
 
 #include "kernels.h"
@@ -34,27 +37,12 @@ constexpr uint32_t kTmemCols = 256, kTmemS = 0, kTmemO = 64, kTmemP = 192;  // P
 constexpr uint32_t kAtom = kKeys * 128;                                     // 64 rows x 128 bytes
 constexpr int kNoChunk = 0x7fffffff;
 
-template <int D>
-struct VarlenSmem {
-  static constexpr int kStages = D == 64 ? 4 : 2;
-  alignas(1024) uint8_t q[D / 64][kRows * 128];
-  alignas(1024) uint8_t k[kStages][D / 64][kAtom];
-  alignas(1024) uint8_t v[kStages][D / 64][kAtom];
-  uint32_t docs[kDocWords];
-  int doc_lo[4], doc_hi[4];
-  alignas(8) uint64_t qfull, kfull[kStages], kempty[kStages], vfull[kStages], vempty[kStages];
-  uint64_t sfull, sfree, pfull[2], pfree[2], drain;
-  uint32_t tmem;
-  int abort;
-};
-template <int D>
-constexpr size_t smem_bytes() { return sizeof(VarlenSmem<D>) + 1024; }
+constexpr int kRing = 3;  // units published ahead
 
-// The chunks of a CTA: [0, end_a) of the prefix and [beg_b, end_b) of the window, cut to [lo, hi).
+// The chunks of a unit: [0, end_a) of the prefix and [beg_b, end_b) of the window, cut to [lo, hi).
 struct Chunks {
   int end_a, beg_b, lo, hi;
-  const uint32_t* docs;  // or null
-  __device__ __forceinline__ int next(int c) const {
+  __device__ __forceinline__ int next(int c, const uint32_t* docs) const {  // docs: the bitmap, or null
     for (++c; c < hi; ++c) {
       if (c >= end_a && c < beg_b) {
         c = beg_b;
@@ -67,8 +55,33 @@ struct Chunks {
     }
     return kNoChunk;
   }
-  __device__ __forceinline__ int first() const { return next(lo - 1); }
 };
+
+struct Unit {
+  Chunks ch;
+  int first;       // its first chunk, or kNoChunk
+  int q_row, rows; // first query row in q, and how many
+  int p0;          // key position of the first
+  int k0, lk, prefix;
+  int h, sp;       // h < 0: no more units
+};
+
+template <int D>
+struct VarlenSmem {
+  static constexpr int kStages = D == 64 ? 4 : 2, kQSlots = D == 64 ? 2 : 1;
+  alignas(1024) uint8_t q[kQSlots][D / 64][kRows * 128];
+  alignas(1024) uint8_t k[kStages][D / 64][kAtom];
+  alignas(1024) uint8_t v[kStages][D / 64][kAtom];
+  uint32_t docs[kRing][kDocWords];
+  Unit units[kRing];
+  alignas(8) uint64_t ufull[kRing], uempty[kRing];
+  uint64_t qfull[kQSlots], qempty[kQSlots], kfull[kStages], kempty[kStages], vfull[kStages], vempty[kStages];
+  uint64_t sfull, sfree, pfull[2], pfree[2], drain;
+  uint32_t tmem;
+  int abort;
+};
+template <int D>
+constexpr size_t smem_bytes() { return sizeof(VarlenSmem<D>) + 1024; }
 
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, int* err, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err, code));
@@ -80,35 +93,27 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// MOD: scores are capped or biased by distance.
-template <int D, bool MOD>
+// MOD: scores are capped or biased by distance. BF: bf16, else fp16.
+template <int D, bool MOD, bool BF>
 __global__ void __launch_bounds__(kThreads, 2)
     varlen_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                     const __grid_constant__ CUtensorMap tv, const VarlenArgs a, int* err) {
+                     const __grid_constant__ CUtensorMap tv, const VarlenArgs a, int nunits, int* err) {
   using Smem = VarlenSmem<D>;
-  constexpr int kStages = Smem::kStages, kAtoms = D / 64;
-  pdl_trigger();
-  pdl_wait();
-  // block -> (tile, sequence, head, split), the tile slowest and last first
-  int u = static_cast<int>(blockIdx.x);
-  const int sp = u % a.splits;
-  u /= a.splits;
-  const int h = u % a.Hq;
-  u /= a.Hq;
-  const int b = u % a.B;
-  const int tiles = (a.max_q + kRows - 1) / kRows;
-  const int t0 = (tiles - 1 - u / a.B) * kRows;
-  const Sequence s = sequence(a, b);
-  if (t0 >= min(s.lq, a.max_q)) return;
-
+  constexpr int kStages = Smem::kStages, kAtoms = D / 64, kQSlots = Smem::kQSlots;
+  constexpr int kType = BF ? DT_BF16 : DT_F16;
   extern __shared__ uint8_t smem_raw[];
   Smem& S = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rows = min(kRows, min(s.lq, a.max_q) - t0);  // query rows of this CTA
-  const int p0 = t0 + s.lk - s.lq;                       // key position of its first row
-
+  pdl_trigger();
   if (threadIdx.x == 0) {
-    mbar_init(smem_u32(&S.qfull), 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(smem_u32(&S.ufull[i]), 1);
+      mbar_init(smem_u32(&S.uempty[i]), 5);  // the MMA issuer and the four softmax warps
+    }
+    for (int i = 0; i < kQSlots; ++i) {
+      mbar_init(smem_u32(&S.qfull[i]), 1);
+      mbar_init(smem_u32(&S.qempty[i]), 1);
+    }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&S.kfull[i]), 1);
       mbar_init(smem_u32(&S.kempty[i]), 1);
@@ -127,128 +132,195 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   if (warp == 0 && lane == 0) { tma_prefetch_desc(&tq); tma_prefetch_desc(&tk); tma_prefetch_desc(&tv); }
   if (warp == 1) { tmem_alloc(smem_u32(&S.tmem), kTmemCols); tmem_relinquish(); }
-  // row of this thread (softmax warps): TMEM lanes 32 * (warp % 4) .. belong to warp
-  const int qw = warp & 3, row = qw * 32 + lane;
-  int qdoc = 0;
-  if (a.doc_q) {
-    for (int i = threadIdx.x; i < kDocWords; i += kThreads) S.docs[i] = 0u;
-  }
-  if (a.doc_q && warp >= 2) {
-    qdoc = row < rows ? a.doc_q[s.q0 + t0 + row] : -1;
-    const int lo = __reduce_min_sync(0xffffffffu, qdoc < 0 ? 0x7fffffff : qdoc);
-    const int hi = __reduce_max_sync(0xffffffffu, qdoc);
-    if (lane == 0) { S.doc_lo[qw] = lo; S.doc_hi[qw] = hi; }
-  }
-
-  Chunks ch;
-  {
-    const int wlo = max(0, p0 - a.left), whi = min(s.lk, p0 + rows - 1 + a.right + 1);
-    ch.end_a = (s.prefix + kKeys - 1) / kKeys;
-    ch.beg_b = whi > wlo ? wlo / kKeys : ch.end_a;
-    const int end_b = whi > wlo ? (whi + kKeys - 1) / kKeys : 0;
-    const int lo = ch.end_a > 0 ? 0 : ch.beg_b, hi = max(ch.end_a, end_b);
-    const long long n = max(0, hi - lo);
-    ch.lo = lo + static_cast<int>(n * sp / a.splits);
-    ch.hi = lo + static_cast<int>(n * (sp + 1) / a.splits);
-    ch.docs = a.doc_k ? S.docs : nullptr;
-  }
-  if (a.doc_k) {
-    __syncthreads();
-    const int lo = min(min(S.doc_lo[0], S.doc_lo[1]), min(S.doc_lo[2], S.doc_lo[3]));
-    const int hi = max(max(S.doc_hi[0], S.doc_hi[1]), max(S.doc_hi[2], S.doc_hi[3]));
-    const int* ids = a.doc_k + s.k0;
-    const int end = min(ch.hi, kDocWords * 32);
-#pragma unroll 4
-    for (int c = ch.lo + warp; c < end; c += kThreads / 32) {
-      const int k = c * kKeys + lane;
-      const int x = k < s.lk ? ids[k] : -1, y = k + 32 < s.lk ? ids[k + 32] : -1;
-      const bool hit = (x >= lo && x <= hi && x >= 0) || (y >= lo && y <= hi && y >= 0);
-      if (__any_sync(0xffffffffu, hit) && lane == 0) atomicOr(&S.docs[c >> 5], 1u << (c & 31));
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = S.tmem;
+  pdl_wait();
   volatile int* abort = &S.abort;
+  const bool docs = a.doc_k != nullptr;
 
   if (warp == 0) {
-    if (lane == 0) {
-      const int hk = h / (a.Hq / a.Hkv);
-      int nk = 0, nv = 0, nq = 0, c = ch.first();
-      if (c != kNoChunk) {
-        mbar_expect_tx(smem_u32(&S.qfull), kRows * D * 2);
-#pragma unroll
-        for (int d = 0; d < kAtoms; ++d) tma_load_3d(smem_u32(S.q[d]), &tq, d * 64, h, s.q0 + t0, smem_u32(&S.qfull));
-        ++nq;
+    // ---------------- producer. Counters run over all units: n chunks, nq Q tiles, nu published units.
+    const int tiles = (a.max_q + kRows - 1) / kRows;
+    int n = 0, nk = 0, nv = 0, nq = 0, nu = 0;
+    bool ok = true;
+    for (int w = static_cast<int>(blockIdx.x); ok; w += static_cast<int>(gridDim.x)) {
+      // unit -> (tile, sequence, head, range), the tile slowest and last first
+      Unit u;
+      u.h = -1;
+      if (w < nunits) {
+        int x = w;
+        u.sp = x % a.splits;
+        x /= a.splits;
+        const int h = x % a.Hq;
+        x /= a.Hq;
+        const Sequence s = sequence(a, x % a.B);
+        const int t0 = (tiles - 1 - x / a.B) * kRows, lq = min(s.lq, a.max_q);
+        if (t0 >= lq) continue;
+        u.h = h;
+        u.rows = min(kRows, lq - t0);
+        u.q_row = s.q0 + t0;
+        u.p0 = t0 + s.lk - s.lq;
+        u.k0 = s.k0;
+        u.lk = s.lk;
+        u.prefix = s.prefix;
+        const int wlo = max(0, u.p0 - a.left), whi = min(s.lk, u.p0 + u.rows - 1 + a.right + 1);
+        u.ch.end_a = (s.prefix + kKeys - 1) / kKeys;
+        u.ch.beg_b = whi > wlo ? wlo / kKeys : u.ch.end_a;
+        const int end_b = whi > wlo ? (whi + kKeys - 1) / kKeys : 0;
+        const int lo = u.ch.end_a > 0 ? 0 : u.ch.beg_b;
+        const long long all = max(0, max(u.ch.end_a, end_b) - lo);
+        u.ch.lo = lo + static_cast<int>(all * u.sp / a.splits);
+        u.ch.hi = lo + static_cast<int>(all * (u.sp + 1) / a.splits);
       }
-      for (int n = 0; c != kNoChunk; c = ch.next(c), ++n) {
-        const int st = n % kStages, ph = ((n / kStages) - 1) & 1;
-        if (n >= kStages && !mbar_wait(smem_u32(&S.kempty[st]), ph, abort, err, kErrAttnLoad)) break;
-        mbar_expect_tx(smem_u32(&S.kfull[st]), kAtoms * kAtom);
+      const int rs = nu % kRing;
+      uint32_t* map = S.docs[rs];
+      if (nu >= kRing && !warp_wait(smem_u32(&S.uempty[rs]), ((nu / kRing) - 1) & 1, abort, err, kErrAttnLoad)) break;
+      if (docs && u.h >= 0) {
+        // the rows' smallest and largest document, then the chunks that hold a key in that range
+        int lo = 0x7fffffff, hi = -1;
 #pragma unroll
-        for (int d = 0; d < kAtoms; ++d)
-          tma_load_3d(smem_u32(S.k[st][d]), &tk, d * 64, hk, s.k0 + c * kKeys, smem_u32(&S.kfull[st]));
-        ++nk;
-        if (n >= kStages && !mbar_wait(smem_u32(&S.vempty[st]), ph, abort, err, kErrAttnLoad)) break;
-        mbar_expect_tx(smem_u32(&S.vfull[st]), kAtoms * kAtom);
-#pragma unroll
-        for (int d = 0; d < kAtoms; ++d)
-          tma_load_3d(smem_u32(S.v[st][d]), &tv, d * 64, hk, s.k0 + c * kKeys, smem_u32(&S.vfull[st]));
-        ++nv;
-      }
-      if (*abort) {  // the loads in flight land before the CTA can exit
-        const long long t = clock64();
-        auto landed = [&](uint64_t* bar, int issued) {
-          if (issued <= 0) return;
-          while (!mbar_try(smem_u32(bar), (issued - 1) & 1))
-            if (clock64() - t > kWaitBudgetCycles) { atomicCAS(err, 0, kErrGemmDrain); return; }
-        };
-        landed(&S.qfull, nq);
-        for (int i = 0; i < kStages; ++i) {
-          landed(&S.kfull[i], (nk - i + kStages - 1) / kStages);
-          landed(&S.vfull[i], (nv - i + kStages - 1) / kStages);
+        for (int i = 0; i < kRows; i += 32) {
+          const int d = lane + i < u.rows ? a.doc_q[u.q_row + lane + i] : -1;
+          lo = min(lo, d < 0 ? 0x7fffffff : d);
+          hi = max(hi, d);
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        const int* ids = a.doc_k + u.k0;
+        const int end = min(u.ch.hi, kDocWords * 32);
+        for (int c0 = u.ch.lo & ~31; c0 < end; c0 += 32) {
+          uint32_t word = 0;
+          const int c1 = min(c0 + 32, end);
+#pragma unroll 8
+          for (int c = max(c0, u.ch.lo); c < c1; ++c) {
+            const int k = c * kKeys + lane;
+            const int x = k < u.lk ? ids[k] : -1, y = k + 32 < u.lk ? ids[k + 32] : -1;
+            const bool hit = (x >= lo && x <= hi && x >= 0) || (y >= lo && y <= hi && y >= 0);
+            if (__any_sync(0xffffffffu, hit)) word |= 1u << (c & 31);
+          }
+          if (lane == 0) map[c0 >> 5] = word;
         }
       }
+      __syncwarp();
+      int c = kNoChunk;
+      if (u.h >= 0) c = u.ch.next(u.ch.lo - 1, docs ? map : nullptr);
+      u.first = c;
+      if (lane == 0) {
+        S.units[rs] = u;
+        mbar_arrive(smem_u32(&S.ufull[rs]));
+      }
+      __syncwarp();
+      ++nu;
+      if (u.h < 0) break;
+      if (c == kNoChunk) continue;
+      const int hk = u.h / (a.Hq / a.Hkv);
+      if (lane == 0) {
+        const int qs = nq % kQSlots;
+        ok = nq < kQSlots || mbar_wait(smem_u32(&S.qempty[qs]), ((nq / kQSlots) - 1) & 1, abort, err, kErrAttnLoad);
+        if (ok) {
+          mbar_expect_tx(smem_u32(&S.qfull[qs]), kRows * D * 2);
+#pragma unroll
+          for (int d = 0; d < kAtoms; ++d)
+            tma_load_3d(smem_u32(S.q[qs][d]), &tq, d * 64, u.h, u.q_row, smem_u32(&S.qfull[qs]));
+          ++nq;
+        }
+        for (; ok && c != kNoChunk; c = u.ch.next(c, docs ? map : nullptr), ++n) {
+          const int st = n % kStages, ph = ((n / kStages) - 1) & 1;
+          if (n >= kStages && !mbar_wait(smem_u32(&S.kempty[st]), ph, abort, err, kErrAttnLoad)) { ok = false; break; }
+          mbar_expect_tx(smem_u32(&S.kfull[st]), kAtoms * kAtom);
+#pragma unroll
+          for (int d = 0; d < kAtoms; ++d)
+            tma_load_3d(smem_u32(S.k[st][d]), &tk, d * 64, hk, u.k0 + c * kKeys, smem_u32(&S.kfull[st]));
+          ++nk;
+          if (n >= kStages && !mbar_wait(smem_u32(&S.vempty[st]), ph, abort, err, kErrAttnLoad)) { ok = false; break; }
+          mbar_expect_tx(smem_u32(&S.vfull[st]), kAtoms * kAtom);
+#pragma unroll
+          for (int d = 0; d < kAtoms; ++d)
+            tma_load_3d(smem_u32(S.v[st][d]), &tv, d * 64, hk, u.k0 + c * kKeys, smem_u32(&S.vfull[st]));
+          ++nv;
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
     }
+    if (lane == 0 && *abort) {  // the loads in flight land before the CTA can exit
+      const long long t = clock64();
+      auto landed = [&](uint64_t* bar, int issued) {
+        if (issued <= 0) return;
+        while (!mbar_try(smem_u32(bar), (issued - 1) & 1))
+          if (clock64() - t > kWaitBudgetCycles) { atomicCAS(err, 0, kErrGemmDrain); return; }
+      };
+      for (int i = 0; i < kQSlots; ++i) landed(&S.qfull[i], (nq - i + kQSlots - 1) / kQSlots);
+      for (int i = 0; i < kStages; ++i) {
+        landed(&S.kfull[i], (nk - i + kStages - 1) / kStages);
+        landed(&S.vfull[i], (nv - i + kStages - 1) / kStages);
+      }
+    }
+    __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t fmt = a.type == DT_BF16 ? 1u : 0u;
-      const uint32_t idesc = idesc_of(fmt, kRows, kKeys), idesc_pv = idesc_of(fmt, kRows, 64) | (1u << 16);
-      bool issued = false;
-      int c = ch.first(), n = 0;
-      // O += P V of chunk m; V's atoms of 64 columns are separate products
-      auto pv = [&](int m) -> bool {
-        const int st = m % kStages, pb = m & 1;
-        if (!mbar_wait(smem_u32(&S.pfull[pb]), (m >> 1) & 1, abort, err, kErrAttnMma)) return false;
-        if (!mbar_wait(smem_u32(&S.vfull[st]), (m / kStages) & 1, abort, err, kErrAttnMma)) return false;
+      const uint32_t idesc = idesc_of(BF ? 1u : 0u, kRows, kKeys), idesc_pv = idesc_of(BF ? 1u : 0u, kRows, 64) | (1u << 16);
+      bool issued = false, ok = true;
+      int n = 0, nq = 0, nu = 0;
+      int pend = -1;           // chunk whose product with V is still to be issued
+      bool pend_first = false; // it starts its unit's O
+      uint32_t pend_o = kTmemO;
+      // O += P V of the pending chunk; V's atoms of 64 columns are separate products
+      auto pv = [&]() -> bool {
+        const int st = pend % kStages, pb = pend & 1;
+        if (!mbar_wait(smem_u32(&S.pfull[pb]), (pend >> 1) & 1, abort, err, kErrAttnMma)) return false;
+        if (!mbar_wait(smem_u32(&S.vfull[st]), (pend / kStages) & 1, abort, err, kErrAttnMma)) return false;
         tc_fence_after();
 #pragma unroll
         for (int d = 0; d < kAtoms; ++d)
 #pragma unroll
           for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys: 8 packed columns of P
-            umma_bf16_ts(tmem + kTmemO + 64 * d, tmem + kTmemP + pb * 32 + kk * 8,
-                         sdesc_mn128(smem_u32(S.v[st][d]) + kk * 2048), idesc_pv, (m > 0 || kk > 0) ? 1u : 0u);
+            umma_bf16_ts(tmem + pend_o + 64 * d, tmem + kTmemP + pb * 32 + kk * 8,
+                         sdesc_mn128(smem_u32(S.v[st][d]) + kk * 2048), idesc_pv, (!pend_first || kk > 0) ? 1u : 0u);
         umma_commit(smem_u32(&S.pfree[pb]));
         umma_commit(smem_u32(&S.vempty[st]));
+        pend = -1;
         return true;
       };
-      bool ok = c == kNoChunk || mbar_wait(smem_u32(&S.qfull), 0, abort, err, kErrAttnMma);
-      for (; ok && c != kNoChunk; c = ch.next(c), ++n) {
-        const int st = n % kStages;
-        if (!mbar_wait(smem_u32(&S.kfull[st]), (n / kStages) & 1, abort, err, kErrAttnMma)) { ok = false; break; }
-        if (n >= 1 && !mbar_wait(smem_u32(&S.sfree), (n - 1) & 1, abort, err, kErrAttnMma)) { ok = false; break; }
-        tc_fence_after();
+      for (;; ++nu) {
+        const int rs = nu % kRing;
+        if (!mbar_wait(smem_u32(&S.ufull[rs]), (nu / kRing) & 1, abort, err, kErrAttnMma)) { ok = false; break; }
+        const Unit& u = S.units[rs];
+        if (u.h < 0) break;
+        int c = u.first;
+        if (c != kNoChunk) {
+          const int qs = nq % kQSlots;
+          if (!mbar_wait(smem_u32(&S.qfull[qs]), (nq / kQSlots) & 1, abort, err, kErrAttnMma)) { ok = false; break; }
+          for (; c != kNoChunk; ++n) {
+            const int st = n % kStages;
+            if (!mbar_wait(smem_u32(&S.kfull[st]), (n / kStages) & 1, abort, err, kErrAttnMma)) { ok = false; break; }
+            // the softmax warps have copied the previous scores
+            if (n >= 1 && !mbar_wait(smem_u32(&S.sfree), (n - 1) & 1, abort, err, kErrAttnMma)) { ok = false; break; }
+            tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tmem + kTmemS, sdesc_k128(smem_u32(S.q[kk / 4]) + (kk % 4) * 32),
-                    sdesc_k128(smem_u32(S.k[st][kk / 4]) + (kk % 4) * 32), idesc, kk > 0 ? 1u : 0u);
-        issued = true;
-        umma_commit(smem_u32(&S.sfull));
-        umma_commit(smem_u32(&S.kempty[st]));
-        if (n >= 1 && !pv(n - 1)) ok = false;
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_bf16(tmem + kTmemS, sdesc_k128(smem_u32(S.q[qs][kk / 4]) + (kk % 4) * 32),
+                        sdesc_k128(smem_u32(S.k[st][kk / 4]) + (kk % 4) * 32), idesc, kk > 0 ? 1u : 0u);
+            issued = true;
+            umma_commit(smem_u32(&S.sfull));
+            umma_commit(smem_u32(&S.kempty[st]));
+            const bool is_first = c == u.first;
+            c = u.ch.next(c, docs ? S.docs[rs] : nullptr);
+            if (c == kNoChunk) umma_commit(smem_u32(&S.qempty[qs]));
+            if (pend >= 0 && !pv()) { ok = false; break; }
+            pend = n;
+            pend_first = is_first;
+            pend_o = kTmemO + (D == 64 ? static_cast<uint32_t>(nq & 1) * 64u : 0u);
+          }
+          if (!ok) break;
+          ++nq;
+        }
+        // a unit without chunks: the softmax warps write the previous one out first
+        if (c == kNoChunk && u.first == kNoChunk && pend >= 0 && !pv()) { ok = false; break; }
+        mbar_arrive(smem_u32(&S.uempty[rs]));
       }
-      if (ok && n > 0) pv(n - 1);
+      if (ok && pend >= 0) pv();
       if (*abort && issued) {  // the products already issued finish before TMEM is released
         umma_commit(smem_u32(&S.drain));
         const long long t = clock64();
@@ -258,219 +330,265 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else {
     // ---------------- softmax: scores stay in units of q.k until the exponential scales them
+    const int qw = warp & 3, row = qw * 32 + lane;  // this thread's row; warp w owns TMEM lanes 32 (w % 4) ..
     const uint32_t tl = tmem + (static_cast<uint32_t>(qw * 32) << 16);
     const float cs = a.scale * kLog2e;
-    const float cap_in = a.cap > 0.f ? a.scale / a.cap : 0.f, cap_out = a.cap / a.scale;
-    const float slope = MOD && a.slopes ? a.slopes[h] / a.scale : 0.f;
-    const int p = p0 + row;             // this row's key position
-    const int pw = p0 + qw * 32;        // the warp's first and last
-    const int pz = pw + 31;
-    float m_used = -INFINITY;
-    float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
+    const float cap_in = MOD && a.cap > 0.f ? a.scale / a.cap : 0.f, cap_out = MOD ? a.cap / a.scale : 0.f;
+    int n = 0, nq = 0, nu = 0;
     bool ok = true;
-    int c = ch.first(), n = 0;
-    int kid[2] = {0, 0};
-    auto load_ids = [&](int chunk) {
-      if (!a.doc_k || chunk == kNoChunk) return;
+
+    // one thread's output row, written once its unit's last product has landed
+    struct Row {
+      bool on;          // a unit's row is waiting
+      int chunk;        // its last chunk
+      uint32_t o;       // its TMEM columns
+      long long at;     // row in q; -1: none
+      int h, sp;
+      float inv, lse2;
+    } wait{false, 0, 0, 0, 0, 0, 0.f, 0.f};
+    auto put = [&](bool zero) {
+      if (wait.at >= 0) {
+        if (a.splits == 1) {
+          if (a.lse) a.lse[wait.at * a.Hq + wait.h] = wait.lse2 * kLn2;
+        } else {
+          a.part_l[(static_cast<long long>(wait.sp) * a.rows_q + wait.at) * a.Hq + wait.h] = wait.lse2;
+        }
+      }
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int k = chunk * kKeys + 32 * g + lane;
-        kid[g] = k < s.lk ? a.doc_k[s.k0 + k] : -1;
+      for (int d = 0; d < D / 32; ++d) {
+        float o[32];
+        if (zero) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        } else {
+          tmem_ld32(tl + wait.o + 32 * d, o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] *= wait.inv;
+        }
+        if (wait.at < 0) continue;
+        if (a.splits == 1) {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + wait.at * a.ldo + wait.h * D) + 4 * d;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            dst[j] = make_uint4(pack_pair(o[8 * j], o[8 * j + 1], kType), pack_pair(o[8 * j + 2], o[8 * j + 3], kType),
+                                pack_pair(o[8 * j + 4], o[8 * j + 5], kType), pack_pair(o[8 * j + 6], o[8 * j + 7], kType));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(
+              a.part_o + ((static_cast<long long>(wait.sp) * a.rows_q + wait.at) * a.Hq + wait.h) * D + 32 * d);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
       }
     };
-    load_ids(c);
-    while (c != kNoChunk) {
-      const int k0 = c * kKeys, pb = n & 1, st = n % kStages;
-      // per 32-key group, warp-uniform: 0 nobody sees a key, 1 some are masked, 2 all are seen
-      int gk[2];
-      bool dead = k0 + kKeys > s.lk;  // the chunk holds keys that nobody may see
-      bool same[2] = {true, true};
-      const int kd[2] = {kid[0], kid[1]};
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int k_lo = k0 + 32 * g, k_hi = k_lo + 31;
-        const bool none = k_lo >= s.lk || ((k_hi < pw - a.left || k_lo > pz + a.right) && k_lo >= s.prefix);
-        const bool all = k_hi < s.lk && ((k_lo >= pz - a.left && k_hi <= pw + a.right) || k_hi < s.prefix);
-        gk[g] = none ? 0 : all ? 2 : 1;
-        if (a.doc_k) {
-          dead = dead || __any_sync(0xffffffffu, kd[g] < 0);
-          const int d0 = __shfl_sync(0xffffffffu, qdoc, 0);
-          same[g] = __all_sync(0xffffffffu, kd[g] == d0 && qdoc == d0 && d0 >= 0);
-          if (!same[g] && gk[g] == 2) gk[g] = 1;
-        }
-      }
-      const int c_next = ch.next(c);
-      load_ids(c_next);
-      if (!warp_wait(smem_u32(&S.sfull), n & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
+    auto flush = [&]() -> bool {
+      if (!wait.on) return true;
+      wait.on = false;
+      if (!warp_wait(smem_u32(&S.pfree[wait.chunk & 1]), (wait.chunk >> 1) & 1, abort, err, kErrAttnSoftmax)) return false;
       tc_fence_after();
-      float x[64];
-      tmem_ld64(tl + kTmemS, x);
+      put(false);
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&S.sfree));  // S may take the next chunk
+      return true;
+    };
 
-      if constexpr (MOD) {
-        if (a.cap > 0.f) {
-          float top = 0.f;
+    for (; ok; ++nu) {
+      const int rs = nu % kRing;
+      if (!warp_wait(smem_u32(&S.ufull[rs]), (nu / kRing) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
+      const Unit& u = S.units[rs];
+      if (u.h < 0) break;
+      const int rows = u.rows, lk = u.lk, k_row = u.k0, h = u.h;
+      const int p = u.p0 + row;               // this row's key position
+      const int pw = u.p0 + qw * 32, pz = pw + 31;  // the warp's first and last
+      const long long at = row < rows ? static_cast<long long>(u.q_row) + row : -1;
+      Sequence s;
+      s.lk = lk;
+      s.prefix = u.prefix;
+      const int qdoc = docs && at >= 0 ? a.doc_q[at] : -1;
+      const float slope = MOD && a.slopes ? a.slopes[h] / a.scale : 0.f;
+      const uint32_t* map = docs ? S.docs[rs] : nullptr;
+      const uint32_t oc = kTmemO + (D == 64 ? static_cast<uint32_t>(nq & 1) * 64u : 0u);
+      int c = u.first;
+      if (c == kNoChunk) {  // nothing is seen by any of its rows
+        if (!flush()) { ok = false; break; }
+        wait = Row{false, 0, 0, at, h, u.sp, 0.f, -INFINITY};
+        put(true);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&S.uempty[rs]));
+        continue;
+      }
+      float m_used = -INFINITY;
+      float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
+      int kid[2] = {0, 0};
+      auto load_ids = [&](int chunk) {
+        if (!docs || chunk == kNoChunk) return;
 #pragma unroll
-          for (int i = 0; i < 64; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
-          if (__all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
-            // the polynomial in the squared score, two lanes an instruction
-            const float z1 = cap_in * cap_in, k1 = -z1 / 3.f, k2 = z1 * z1 * (2.f / 15.f),
-                        k3 = z1 * z1 * z1 * (-17.f / 315.f);
-            const float2 c1 = make_float2(k1, k1), c2 = make_float2(k2, k2), c3 = make_float2(k3, k3),
-                         one = make_float2(1.f, 1.f);
+        for (int g = 0; g < 2; ++g) {
+          const int k = chunk * kKeys + 32 * g + lane;
+          kid[g] = k < lk ? a.doc_k[k_row + k] : -1;
+        }
+      };
+      load_ids(c);
+      for (bool first = true; c != kNoChunk; first = false, ++n) {
+        const int k0 = c * kKeys, pb = n & 1, st = n % kStages;
+        // per 32-key group, warp-uniform: 0 nobody sees a key, 1 some are masked, 2 all are seen
+        int gk[2];
+        bool dead = k0 + kKeys > lk;  // the chunk holds keys that nobody may see
+        bool same[2] = {true, true};
+        const int kd[2] = {kid[0], kid[1]};
 #pragma unroll
-            for (int i = 0; i < 64; i += 2) {
-              const float2 v = make_float2(x[i], x[i + 1]), z = __fmul2_rn(v, v);
-              const float2 r = __fmul2_rn(v, __ffma2_rn(z, __ffma2_rn(z, __ffma2_rn(z, c3, c2), c1), one));
-              x[i] = r.x;
-              x[i + 1] = r.y;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) x[i] = cap_out * tanh_any(x[i] * cap_in);
+        for (int g = 0; g < 2; ++g) {
+          const int k_lo = k0 + 32 * g, k_hi = k_lo + 31;
+          const bool none = k_lo >= lk || ((k_hi < pw - a.left || k_lo > pz + a.right) && k_lo >= s.prefix);
+          const bool all = k_hi < lk && ((k_lo >= pz - a.left && k_hi <= pw + a.right) || k_hi < s.prefix);
+          gk[g] = none ? 0 : all ? 2 : 1;
+          if (docs) {
+            dead = dead || __any_sync(0xffffffffu, kd[g] < 0);
+            const int d0 = __shfl_sync(0xffffffffu, qdoc, 0);
+            same[g] = __all_sync(0xffffffffu, kd[g] == d0 && qdoc == d0 && d0 >= 0);
+            if (!same[g] && gk[g] == 2) gk[g] = 1;
           }
         }
-        if (a.slopes) {
-          const float away = static_cast<float>(p - k0);
+        const int c_next = u.ch.next(c, map);
+        load_ids(c_next);
+        if (!warp_wait(smem_u32(&S.sfull), n & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
+        tc_fence_after();
+        float x[64];
+        tmem_ld64(tl + kTmemS, x);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&S.sfree));  // S may take the next chunk
+
+        if constexpr (MOD) {
+          if (a.cap > 0.f) {
+            float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) x[i] = fmaf(-slope, fabsf(away - static_cast<float>(i)), x[i]);
+            for (int i = 0; i < 64; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
+            if (__all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
+              // the polynomial in the squared score, two lanes an instruction
+              const float z1 = cap_in * cap_in, k1 = -z1 / 3.f, k2 = z1 * z1 * (2.f / 15.f),
+                          k3 = z1 * z1 * z1 * (-17.f / 315.f);
+              const float2 c1 = make_float2(k1, k1), c2 = make_float2(k2, k2), c3 = make_float2(k3, k3),
+                           one = make_float2(1.f, 1.f);
+#pragma unroll
+              for (int i = 0; i < 64; i += 2) {
+                const float2 v = make_float2(x[i], x[i + 1]), z = __fmul2_rn(v, v);
+                const float2 r = __fmul2_rn(v, __ffma2_rn(z, __ffma2_rn(z, __ffma2_rn(z, c3, c2), c1), one));
+                x[i] = r.x;
+                x[i + 1] = r.y;
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) x[i] = cap_out * tanh_any(x[i] * cap_in);
+            }
+          }
+          if (a.slopes) {
+            const float away = static_cast<float>(p - k0);
+#pragma unroll
+            for (int i = 0; i < 64; ++i) x[i] = fmaf(-slope, fabsf(away - static_cast<float>(i)), x[i]);
+          }
         }
-      }
-      float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (gk[g] == 1) {
-          uint32_t see = window_bits(a, s, p, k0 + 32 * g);
-          if (a.doc_k && !same[g]) {
-            uint32_t mine = 0;
+        for (int g = 0; g < 2; ++g) {
+          if (gk[g] == 1) {
+            uint32_t see = window_bits(a, s, p, k0 + 32 * g);
+            if (docs && !same[g]) {
+              uint32_t mine = 0;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                mine |= __shfl_sync(0xffffffffu, kd[g], i) == qdoc ? 1u << i : 0u;
+              see = qdoc >= 0 ? see & mine : 0u;
+            }
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              mine |= __shfl_sync(0xffffffffu, kd[g], i) == qdoc ? 1u << i : 0u;
-            see = qdoc >= 0 ? see & mine : 0u;
+              if (!(see >> i & 1)) x[32 * g + i] = -INFINITY;
           }
+          if (gk[g] != 0) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!(see >> i & 1)) x[32 * g + i] = -INFINITY;
-        }
-        if (gk[g] != 0) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) mq[(i >> 1) & 3] = max3(mq[(i >> 1) & 3], x[32 * g + i], x[32 * g + i + 1]);
-        }
-      }
-      const float mx = max3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * cs;
-      const float m_new = fmaxf(m_used, mx);
-      const bool resc = m_new > m_used + 8.f;
-      const bool resc_o = resc && m_used != -INFINITY;  // O is exactly 0 before a row's first visible key
-      float alpha = 1.f;
-      if (resc) {
-        alpha = exp2_fast(m_used - m_new);
-        la.x *= alpha; la.y *= alpha; lb.x *= alpha; lb.y *= alpha;
-        m_used = m_new;
-      }
-      const float msub = m_used == -INFINITY ? 0.f : m_used;
-      const float2 mul2 = make_float2(cs, cs), nm2 = make_float2(-msub, -msub);
-      uint32_t pk[32];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (gk[g] == 0) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pk[16 * g + i] = 0u;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 e = __ffma2_rn(make_float2(x[32 * g + 2 * i], x[32 * g + 2 * i + 1]), mul2, nm2);
-            const float2 pp = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-            if (i & 1) lb = __fadd2_rn(lb, pp); else la = __fadd2_rn(la, pp);
-            pk[16 * g + i] = pack_pair(pp.x, pp.y, a.type);
+            for (int i = 0; i < 32; i += 2) mq[(i >> 1) & 3] = max3(mq[(i >> 1) & 3], x[32 * g + i], x[32 * g + i + 1]);
           }
         }
-      }
-      if (dead) {
-        // V rows of keys that nobody may see: zero, whatever they hold (all four warps, 16 rows each)
-        if (!warp_wait(smem_u32(&S.vfull[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
-        const int r0 = 16 * qw + (lane >> 1);
-        const int k = k0 + r0;
-        const int src = __shfl_sync(0xffffffffu, qw < 2 ? kd[0] : kd[1], r0 & 31);
-        if (k >= s.lk || (a.doc_k && src < 0)) {
+        const float mx = max3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * cs;
+        const float m_new = fmaxf(m_used, mx);
+        const bool resc = m_new > m_used + 8.f;
+        const bool resc_o = resc && m_used != -INFINITY;  // O is exactly 0 before a row's first visible key
+        float alpha = 1.f;
+        if (resc) {
+          alpha = exp2_fast(m_used - m_new);
+          la.x *= alpha; la.y *= alpha; lb.x *= alpha; lb.y *= alpha;
+          m_used = m_new;
+        }
+        const float msub = m_used == -INFINITY ? 0.f : m_used;
+        const float2 mul2 = make_float2(cs, cs), nm2 = make_float2(-msub, -msub);
+        uint32_t pk[32];
 #pragma unroll
-          for (int d = 0; d < kAtoms; ++d) {
-            uint4* z = reinterpret_cast<uint4*>(S.v[st][d] + r0 * 128 + (lane & 1) * 64);
+        for (int g = 0; g < 2; ++g) {
+          if (gk[g] == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < 16; ++i) pk[16 * g + i] = 0u;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 e = __ffma2_rn(make_float2(x[32 * g + 2 * i], x[32 * g + 2 * i + 1]), mul2, nm2);
+              const float2 pp = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+              if (i & 1) lb = __fadd2_rn(lb, pp); else la = __fadd2_rn(la, pp);
+              pk[16 * g + i] = pack_pair(pp.x, pp.y, kType);
+            }
           }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor core reads V
-      }
-      // O may be rescaled once the product in flight has landed
-      if (n > 0 && __any_sync(0xffffffffu, resc_o)) {
-        if (!warp_wait(smem_u32(&S.pfree[(n - 1) & 1]), ((n - 1) >> 1) & 1, abort, err, kErrAttnSoftmax)) {
+        if (dead) {
+          // V rows of keys that nobody may see: zero, whatever they hold (all four warps, 16 rows each)
+          if (!warp_wait(smem_u32(&S.vfull[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
+          const int r0 = 16 * qw + (lane >> 1);
+          const int src = __shfl_sync(0xffffffffu, qw < 2 ? kd[0] : kd[1], r0 & 31);
+          if (k0 + r0 >= lk || (docs && src < 0)) {
+#pragma unroll
+            for (int d = 0; d < kAtoms; ++d) {
+              uint4* z = reinterpret_cast<uint4*>(S.v[st][d] + r0 * 128 + (lane & 1) * 64);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) z[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor core reads V
+        }
+        // O may be rescaled once the product in flight has landed
+        if (!first && __any_sync(0xffffffffu, resc_o)) {
+          if (!warp_wait(smem_u32(&S.pfree[(n - 1) & 1]), ((n - 1) >> 1) & 1, abort, err, kErrAttnSoftmax)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d) {
+            float o[32];
+            tmem_ld32(tl + oc + 32 * d, o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= alpha;
+            tmem_st32(tl + oc + 32 * d, o);
+          }
+        }
+        if (n >= 2 && !warp_wait(smem_u32(&S.pfree[pb]), ((n >> 1) - 1) & 1, abort, err, kErrAttnSoftmax)) {
           ok = false;
           break;
         }
         tc_fence_after();
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-          float o[32];
-          tmem_ld32(tl + kTmemO + 32 * d, o);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] *= alpha;
-          tmem_st32(tl + kTmemO + 32 * d, o);
-        }
+        tmem_st32u(tl + kTmemP + pb * 32, pk);
+        // with one O buffer the previous unit's O leaves before this unit's first product
+        if (D == 128 && first && !flush()) { ok = false; break; }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&S.pfull[pb]));
+        if (D == 64 && first && !flush()) { ok = false; break; }
+        c = c_next;
       }
-      if (n >= 2 && !warp_wait(smem_u32(&S.pfree[pb]), ((n >> 1) - 1) & 1, abort, err, kErrAttnSoftmax)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      tmem_st32u(tl + kTmemP + pb * 32, pk);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&S.pfull[pb]));
-      c = c_next;
-      ++n;
-    }
-    if (ok && n > 0) ok = warp_wait(smem_u32(&S.pfree[(n - 1) & 1]), ((n - 1) >> 1) & 1, abort, err, kErrAttnSoftmax);
-    if (ok) {
-      tc_fence_after();
+      if (!ok) break;
       const float l = (la.x + la.y) + (lb.x + lb.y);
-      const float inv = l > 0.f ? 1.f / l : l;  // a row that sees nothing is 0; NaN stays NaN
-      const long long r = static_cast<long long>(s.q0) + t0 + row;
-      const float lse2 = l == 0.f ? -INFINITY : m_used + log2f(l);
-      if (a.splits == 1) {
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + r * a.ldo + h * D);
-        if (row < rows && a.lse) a.lse[r * a.Hq + h] = lse2 * kLn2;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-          float o[32];
-          if (n > 0) tmem_ld32(tl + kTmemO + 32 * d, o);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = n > 0 ? o[i] * inv : 0.f;
-          if (row < rows) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              dst[4 * d + j] = make_uint4(pack_pair(o[8 * j], o[8 * j + 1], a.type), pack_pair(o[8 * j + 2], o[8 * j + 3], a.type),
-                                          pack_pair(o[8 * j + 4], o[8 * j + 5], a.type), pack_pair(o[8 * j + 6], o[8 * j + 7], a.type));
-          }
-        }
-      } else {
-        const long long at = (static_cast<long long>(sp) * a.rows_q + r) * a.Hq + h;
-        float4* dst = reinterpret_cast<float4*>(a.part_o + at * D);
-        if (row < rows) a.part_l[at] = lse2;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-          float o[32];
-          if (n > 0) tmem_ld32(tl + kTmemO + 32 * d, o);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = n > 0 ? o[i] * inv : 0.f;
-          if (row < rows) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dst[8 * d + j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-          }
-        }
-      }
+      // a row that sees nothing is 0; NaN stays NaN
+      wait = Row{true, n - 1, oc, at, h, u.sp, l > 0.f ? 1.f / l : l, l == 0.f ? -INFINITY : m_used + log2f(l)};
+      ++nq;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&S.uempty[rs]));
     }
+    if (ok) flush();
   }
   tc_fence_before();
   __syncwarp();
@@ -518,7 +636,7 @@ __global__ void __launch_bounds__(256) varlen_join_kernel(const VarlenArgs a) {
 }
 
 template <int D>
-cudaError_t launch(const VarlenArgs& a, int* err, cudaStream_t st) {
+cudaError_t launch(const VarlenArgs& a, int num_sms, int* err, cudaStream_t st) {
   CUtensorMap tq, tk, tv;
   auto map = [&](CUtensorMap* m, const void* base, int heads, int rows, long long ld, int box) {
     return make_rows_map(m, base, a.type, D, static_cast<uint64_t>(heads), static_cast<uint64_t>(rows), D,
@@ -527,21 +645,28 @@ cudaError_t launch(const VarlenArgs& a, int* err, cudaStream_t st) {
   if (!map(&tq, a.q, a.Hq, a.rows_q, a.ldq, kRows) || !map(&tk, a.k, a.Hkv, std::max(1, a.rows_k), a.ldk, kKeys) ||
       !map(&tv, a.v, a.Hkv, std::max(1, a.rows_k), a.ldv, kKeys))
     return cudaErrorInvalidValue;
-  const long long grid = (long long)((a.max_q + kRows - 1) / kRows) * a.B * a.Hq * a.splits;
-  if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const dim3 g(static_cast<unsigned>(grid));
+  const long long units = (long long)((a.max_q + kRows - 1) / kRows) * a.B * a.Hq * a.splits;
+  if (units > 0x7fffffffLL - (1 << 20)) return cudaErrorInvalidValue;
+  const dim3 g(static_cast<unsigned>(std::min<long long>(units, 2LL * num_sms)));
+  auto go = [&](auto kernel) {
+    return launch_pdl(kernel, g, dim3(kThreads), smem_bytes<D>(), st, tq, tk, tv, a, static_cast<int>(units), err);
+  };
   if (a.cap > 0.f || a.slopes)
-    return launch_pdl(varlen_tc_kernel<D, true>, g, dim3(kThreads), smem_bytes<D>(), st, tq, tk, tv, a, err);
-  return launch_pdl(varlen_tc_kernel<D, false>, g, dim3(kThreads), smem_bytes<D>(), st, tq, tk, tv, a, err);
+    return a.type == DT_BF16 ? go(varlen_tc_kernel<D, true, true>) : go(varlen_tc_kernel<D, true, false>);
+  return a.type == DT_BF16 ? go(varlen_tc_kernel<D, false, true>) : go(varlen_tc_kernel<D, false, false>);
 }
 
+template <int D, bool MOD, bool BF>
+cudaError_t prepare_one() {
+  return cudaFuncSetAttribute(varlen_tc_kernel<D, MOD, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              static_cast<int>(smem_bytes<D>()));
+}
 template <int D>
 cudaError_t prepare() {
-  const cudaError_t e = cudaFuncSetAttribute(varlen_tc_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem_bytes<D>()));
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(varlen_tc_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              static_cast<int>(smem_bytes<D>()));
+  for (cudaError_t e : {prepare_one<D, false, false>(), prepare_one<D, false, true>(), prepare_one<D, true, false>(),
+                        prepare_one<D, true, true>()})
+    if (e != cudaSuccess) return e;
+  return cudaSuccess;
 }
 
 }  // namespace
@@ -558,14 +683,14 @@ int varlen_splits(int B, int max_q, int max_k, int Hq, int Hkv, int num_sms) {
   const long long units = few ? (long long)B * Hkv * ((max_q * (Hq / Hkv) + 15) / 16)
                               : (long long)B * Hq * ((max_q + kRows - 1) / kRows);
   const long long most = std::max<long long>(1, max_k / (few ? 512 : 4 * kKeys));
-  const long long want = units > 0 ? (few ? 8LL : 2LL) * num_sms / units : 1;
+  const long long want = units > 0 ? (few ? 6LL : 2LL) * num_sms / units : 1;
   return static_cast<int>(std::max<long long>(1, std::min<long long>({want, most, kVarlenMaxSplits})));
 }
 
-cudaError_t varlen_launch(const VarlenArgs& a, int* err, cudaStream_t st) {
+cudaError_t varlen_launch(const VarlenArgs& a, int num_sms, int* err, cudaStream_t st) {
   cudaError_t e = varlen_few_rows(a.max_q, a.Hq, a.Hkv) ? varlen_few_launch(a, err, st)
-                  : a.D == 64                           ? launch<64>(a, err, st)
-                                                        : launch<128>(a, err, st);
+                  : a.D == 64                           ? launch<64>(a, num_sms, err, st)
+                                                        : launch<128>(a, num_sms, err, st);
   if (e != cudaSuccess || a.splits == 1) return e;
   const long long items = (long long)a.max_q * a.Hq;
   const dim3 g(static_cast<unsigned>((items + 7) / 8), static_cast<unsigned>(a.B));

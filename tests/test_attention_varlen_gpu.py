@@ -357,3 +357,15 @@ def test_key_offsets_past_32_bits():
         out = torch.empty_like(q)
         assert attention(q, k, v, out, None, offsets([lq]), offsets([n]), lq, n, 1, 1, D) == 0
         check_sequence(out.view(lq, 1, D), None, q.view(lq, 1, D), k.reshape(n, 1, D), v.reshape(n, 1, D), BF, 0.125)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_tiles_that_see_nothing_between_others(D):
+    """More units than the GPU runs at once, most of them without a visible key: runs of such units
+    between ordinary ones, in every order that a CTA meets them."""
+    import random
+    rng = random.Random(5)
+    lens = [rng.choice([128, 200, 300]) for _ in range(260)]
+    ids = [[-1 if i % 7 else 0] * n for i, n in enumerate(lens)]
+    out, lse = run(lens, D=D, Hq=4, Hkv=2, docs=(ids, ids))
+    assert bool((lse[:lens[0]] > -math.inf).all()) and bool((lse[lens[0]:lens[0] + lens[1]] == -math.inf).all())
