@@ -42,13 +42,20 @@ constexpr int kRing = 3;  // units published ahead
 // The chunks of a unit: [0, end_a) of the prefix and [beg_b, end_b) of the window, cut to [lo, hi).
 struct Chunks {
   int end_a, beg_b, lo, hi;
-  __device__ __forceinline__ int next(int c, const uint32_t* docs) const {  // docs: the bitmap, or null
-    for (++c; c < hi; ++c) {
+  // The chunk after c; DOCS: that the bitmap `docs` has.
+  template <bool DOCS>
+  __device__ __forceinline__ int next(int c, const uint32_t* docs) const {
+    ++c;
+    if constexpr (!DOCS) {
+      if (c >= end_a) c = max(c, beg_b);
+      return c < hi ? c : kNoChunk;
+    }
+    for (; c < hi; ++c) {
       if (c >= end_a && c < beg_b) {
         c = beg_b;
         if (c >= hi) break;
       }
-      if (!docs || c >= kDocWords * 32) return c;
+      if (c >= kDocWords * 32) return c;
       const uint32_t rest = docs[c >> 5] >> (c & 31);
       if (rest & 1) return c;
       if (rest == 0) c |= 31;  // on to the next word
@@ -93,8 +100,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// MOD: scores are capped or biased by distance. BF: bf16, else fp16.
-template <int D, bool MOD, bool BF>
+// MOD: scores are capped or biased by distance. BF: bf16, else fp16. DOCS: with document ids.
+template <int D, bool MOD, bool BF, bool DOCS>
 __global__ void __launch_bounds__(kThreads, 2)
     varlen_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                      const __grid_constant__ CUtensorMap tv, const VarlenArgs a, int nunits, int* err) {
@@ -138,8 +145,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem = S.tmem;
   pdl_wait();
   volatile int* abort = &S.abort;
-  const bool docs = a.doc_k != nullptr;
-
   if (warp == 0) {
     // ---------------- producer. Counters run over all units: n chunks, nq Q tiles, nu published units.
     const int tiles = (a.max_q + kRows - 1) / kRows;
@@ -177,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int rs = nu % kRing;
       uint32_t* map = S.docs[rs];
       if (nu >= kRing && !warp_wait(smem_u32(&S.uempty[rs]), ((nu / kRing) - 1) & 1, abort, err, kErrAttnLoad)) break;
-      if (docs && u.h >= 0) {
+      if (DOCS && u.h >= 0) {
         // the rows' smallest and largest document, then the chunks that hold a key in that range
         int lo = 0x7fffffff, hi = -1;
 #pragma unroll
@@ -205,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       __syncwarp();
       int c = kNoChunk;
-      if (u.h >= 0) c = u.ch.next(u.ch.lo - 1, docs ? map : nullptr);
+      if (u.h >= 0) c = u.ch.next<DOCS>(u.ch.lo - 1, map);
       u.first = c;
       if (lane == 0) {
         S.units[rs] = u;
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             tma_load_3d(smem_u32(S.q[qs][d]), &tq, d * 64, u.h, u.q_row, smem_u32(&S.qfull[qs]));
           ++nq;
         }
-        for (; ok && c != kNoChunk; c = u.ch.next(c, docs ? map : nullptr), ++n) {
+        for (; ok && c != kNoChunk; c = u.ch.next<DOCS>(c, map), ++n) {
           const int st = n % kStages, ph = ((n / kStages) - 1) & 1;
           if (n >= kStages && !mbar_wait(smem_u32(&S.kempty[st]), ph, abort, err, kErrAttnLoad)) { ok = false; break; }
           mbar_expect_tx(smem_u32(&S.kfull[st]), kAtoms * kAtom);
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             umma_commit(smem_u32(&S.sfull));
             umma_commit(smem_u32(&S.kempty[st]));
             const bool is_first = c == u.first;
-            c = u.ch.next(c, docs ? S.docs[rs] : nullptr);
+            c = u.ch.next<DOCS>(c, S.docs[rs]);
             if (c == kNoChunk) umma_commit(smem_u32(&S.qempty[qs]));
             if (pend >= 0 && !pv()) { ok = false; break; }
             pend = n;
@@ -402,9 +407,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       Sequence s;
       s.lk = lk;
       s.prefix = u.prefix;
-      const int qdoc = docs && at >= 0 ? a.doc_q[at] : -1;
+      const int qdoc = DOCS && at >= 0 ? a.doc_q[at] : -1;
       const float slope = MOD && a.slopes ? a.slopes[h] / a.scale : 0.f;
-      const uint32_t* map = docs ? S.docs[rs] : nullptr;
+      const uint32_t* map = S.docs[rs];
+      const Chunks ch = u.ch;
       const uint32_t oc = kTmemO + (D == 64 ? static_cast<uint32_t>(nq & 1) * 64u : 0u);
       int c = u.first;
       if (c == kNoChunk) {  // nothing is seen by any of its rows
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
       int kid[2] = {0, 0};
       auto load_ids = [&](int chunk) {
-        if (!docs || chunk == kNoChunk) return;
+        if (!DOCS || chunk == kNoChunk) return;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const int k = chunk * kKeys + 32 * g + lane;
@@ -440,14 +446,14 @@ __global__ void __launch_bounds__(kThreads, 2)
           const bool none = k_lo >= lk || ((k_hi < pw - a.left || k_lo > pz + a.right) && k_lo >= s.prefix);
           const bool all = k_hi < lk && ((k_lo >= pz - a.left && k_hi <= pw + a.right) || k_hi < s.prefix);
           gk[g] = none ? 0 : all ? 2 : 1;
-          if (docs) {
+          if constexpr (DOCS) {
             dead = dead || __any_sync(0xffffffffu, kd[g] < 0);
             const int d0 = __shfl_sync(0xffffffffu, qdoc, 0);
             same[g] = __all_sync(0xffffffffu, kd[g] == d0 && qdoc == d0 && d0 >= 0);
             if (!same[g] && gk[g] == 2) gk[g] = 1;
           }
         }
-        const int c_next = u.ch.next(c, map);
+        const int c_next = ch.next<DOCS>(c, map);
         load_ids(c_next);
         if (!warp_wait(smem_u32(&S.sfull), n & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
         tc_fence_after();
@@ -491,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int g = 0; g < 2; ++g) {
           if (gk[g] == 1) {
             uint32_t see = window_bits(a, s, p, k0 + 32 * g);
-            if (docs && !same[g]) {
+            if (DOCS && !same[g]) {
               uint32_t mine = 0;
 #pragma unroll
               for (int i = 0; i < 32; ++i)
@@ -540,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (!warp_wait(smem_u32(&S.vfull[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
           const int r0 = 16 * qw + (lane >> 1);
           const int src = __shfl_sync(0xffffffffu, qw < 2 ? kd[0] : kd[1], r0 & 31);
-          if (k0 + r0 >= lk || (docs && src < 0)) {
+          if (k0 + r0 >= lk || (DOCS && src < 0)) {
 #pragma unroll
             for (int d = 0; d < kAtoms; ++d) {
               uint4* z = reinterpret_cast<uint4*>(S.v[st][d] + r0 * 128 + (lane & 1) * 64);
@@ -651,15 +657,26 @@ cudaError_t launch(const VarlenArgs& a, int num_sms, int* err, cudaStream_t st) 
   auto go = [&](auto kernel) {
     return launch_pdl(kernel, g, dim3(kThreads), smem_bytes<D>(), st, tq, tk, tv, a, static_cast<int>(units), err);
   };
-  if (a.cap > 0.f || a.slopes)
-    return a.type == DT_BF16 ? go(varlen_tc_kernel<D, true, true>) : go(varlen_tc_kernel<D, true, false>);
-  return a.type == DT_BF16 ? go(varlen_tc_kernel<D, false, true>) : go(varlen_tc_kernel<D, false, false>);
+  const int which = (a.cap > 0.f || a.slopes ? 4 : 0) + (a.type == DT_BF16 ? 2 : 0) + (a.doc_k ? 1 : 0);
+  switch (which) {
+    case 0: return go(varlen_tc_kernel<D, false, false, false>);
+    case 1: return go(varlen_tc_kernel<D, false, false, true>);
+    case 2: return go(varlen_tc_kernel<D, false, true, false>);
+    case 3: return go(varlen_tc_kernel<D, false, true, true>);
+    case 4: return go(varlen_tc_kernel<D, true, false, false>);
+    case 5: return go(varlen_tc_kernel<D, true, false, true>);
+    case 6: return go(varlen_tc_kernel<D, true, true, false>);
+    default: return go(varlen_tc_kernel<D, true, true, true>);
+  }
 }
 
 template <int D, bool MOD, bool BF>
 cudaError_t prepare_one() {
-  return cudaFuncSetAttribute(varlen_tc_kernel<D, MOD, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              static_cast<int>(smem_bytes<D>()));
+  const int bytes = static_cast<int>(smem_bytes<D>());
+  const cudaError_t e =
+      cudaFuncSetAttribute(varlen_tc_kernel<D, MOD, BF, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(varlen_tc_kernel<D, MOD, BF, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 template <int D>
 cudaError_t prepare() {
