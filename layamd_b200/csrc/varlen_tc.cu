@@ -36,6 +36,7 @@ constexpr int kDocWords = 128;  // bitmap of 4096 chunks; chunks past it are not
 constexpr uint32_t kTmemCols = 256, kTmemS = 0, kTmemO = 64, kTmemP = 192;  // P: two buffers of 32
 constexpr uint32_t kAtom = kKeys * 128;                                     // 64 rows x 128 bytes
 constexpr int kNoChunk = 0x7fffffff;
+constexpr int kMixed = -2, kMixedRows = -3;  // no single document in a chunk, in a warp's rows
 
 constexpr int kRing = 3;  // units published ahead
 
@@ -80,6 +81,10 @@ struct VarlenSmem {
   alignas(1024) uint8_t k[kStages][D / 64][kAtom];
   alignas(1024) uint8_t v[kStages][D / 64][kAtom];
   uint32_t docs[kRing][kDocWords];
+  // per V stage: the chunk's document ids, {the one id that all its keys have or kMixed, whether it
+  // holds keys that nobody may see}
+  alignas(16) int ids[kStages][kKeys];
+  int2 about[kStages];
   Unit units[kRing];
   alignas(8) uint64_t ufull[kRing], uempty[kRing];
   uint64_t qfull[kQSlots], qempty[kQSlots], kfull[kStages], kempty[kStages], vfull[kStages], vempty[kStages];
@@ -231,23 +236,67 @@ __global__ void __launch_bounds__(kThreads, 2)
             tma_load_3d(smem_u32(S.q[qs][d]), &tq, d * 64, u.h, u.q_row, smem_u32(&S.qfull[qs]));
           ++nq;
         }
-        for (; ok && c != kNoChunk; c = u.ch.next<DOCS>(c, map), ++n) {
-          const int st = n % kStages, ph = ((n / kStages) - 1) & 1;
-          if (n >= kStages && !mbar_wait(smem_u32(&S.kempty[st]), ph, abort, err, kErrAttnLoad)) { ok = false; break; }
-          mbar_expect_tx(smem_u32(&S.kfull[st]), kAtoms * kAtom);
+      }
+      auto load_k = [&]() -> bool {  // one lane
+        const int st = n % kStages;
+        if (n >= kStages && !mbar_wait(smem_u32(&S.kempty[st]), ((n / kStages) - 1) & 1, abort, err, kErrAttnLoad))
+          return false;
+        mbar_expect_tx(smem_u32(&S.kfull[st]), kAtoms * kAtom);
 #pragma unroll
-          for (int d = 0; d < kAtoms; ++d)
-            tma_load_3d(smem_u32(S.k[st][d]), &tk, d * 64, hk, u.k0 + c * kKeys, smem_u32(&S.kfull[st]));
-          ++nk;
-          if (n >= kStages && !mbar_wait(smem_u32(&S.vempty[st]), ph, abort, err, kErrAttnLoad)) { ok = false; break; }
-          mbar_expect_tx(smem_u32(&S.vfull[st]), kAtoms * kAtom);
+        for (int d = 0; d < kAtoms; ++d)
+          tma_load_3d(smem_u32(S.k[st][d]), &tk, d * 64, hk, u.k0 + c * kKeys, smem_u32(&S.kfull[st]));
+        ++nk;
+        return true;
+      };
+      auto v_free = [&]() -> bool {
+        return n < kStages || mbar_wait(smem_u32(&S.vempty[n % kStages]), ((n / kStages) - 1) & 1, abort, err, kErrAttnLoad);
+      };
+      auto load_v = [&]() {  // one lane
+        const int st = n % kStages;
+        mbar_expect_tx(smem_u32(&S.vfull[st]), kAtoms * kAtom);
 #pragma unroll
-          for (int d = 0; d < kAtoms; ++d)
-            tma_load_3d(smem_u32(S.v[st][d]), &tv, d * 64, hk, u.k0 + c * kKeys, smem_u32(&S.vfull[st]));
-          ++nv;
+        for (int d = 0; d < kAtoms; ++d)
+          tma_load_3d(smem_u32(S.v[st][d]), &tv, d * 64, hk, u.k0 + c * kKeys, smem_u32(&S.vfull[st]));
+        ++nv;
+      };
+      if constexpr (!DOCS) {
+        if (lane == 0) {
+          for (; ok && c != kNoChunk; c = u.ch.next<false>(c, map), ++n) {
+            ok = load_k() && v_free();
+            if (ok) load_v();
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+      } else {
+        // the chunk's ids and what they have in common go along with V, a chunk ahead in registers
+        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+        int id[2] = {-1, -1};
+        auto load_ids = [&](int chunk) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int k = chunk * kKeys + 32 * g + lane;
+            id[g] = k < u.lk ? a.doc_k[u.k0 + k] : -1;
+          }
+        };
+        load_ids(c);
+        while (ok && c != kNoChunk) {
+          if (lane == 0) ok = load_k();
+          ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+          if (!ok || !__all_sync(0xffffffffu, v_free())) { ok = false; break; }
+          const int st = n % kStages;
+          const int id0 = __shfl_sync(0xffffffffu, id[0], 0);
+          const bool one = __all_sync(0xffffffffu, id[0] == id0 && id[1] == id0);
+          const bool dead = __any_sync(0xffffffffu, id[0] < 0 || id[1] < 0);
+          S.ids[st][lane] = id[0];
+          S.ids[st][lane + 32] = id[1];
+          if (lane == 0) S.about[st] = make_int2(one ? id0 : kMixed, dead ? 1 : 0);
+          __syncwarp();
+          if (lane == 0) load_v();
+          c = u.ch.next<true>(c, map);
+          ++n;
+          if (c != kNoChunk) load_ids(c);
         }
       }
-      ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
     }
     if (lane == 0 && *abort) {  // the loads in flight land before the CTA can exit
       const long long t = clock64();
@@ -400,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (!warp_wait(smem_u32(&S.ufull[rs]), (nu / kRing) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
       const Unit& u = S.units[rs];
       if (u.h < 0) break;
-      const int rows = u.rows, lk = u.lk, k_row = u.k0, h = u.h;
+      const int rows = u.rows, lk = u.lk, h = u.h;
       const int p = u.p0 + row;               // this row's key position
       const int pw = u.p0 + qw * 32, pz = pw + 31;  // the warp's first and last
       const long long at = row < rows ? static_cast<long long>(u.q_row) + row : -1;
@@ -423,38 +472,33 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       float m_used = -INFINITY;
       float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
-      int kid[2] = {0, 0};
-      auto load_ids = [&](int chunk) {
-        if (!DOCS || chunk == kNoChunk) return;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const int k = chunk * kKeys + 32 * g + lane;
-          kid[g] = k < lk ? a.doc_k[k_row + k] : -1;
-        }
-      };
-      load_ids(c);
+      int wdoc = kMixedRows;  // the document of all the warp's rows
+      if constexpr (DOCS) {
+        const int d0 = __shfl_sync(0xffffffffu, qdoc, 0);
+        if (__all_sync(0xffffffffu, qdoc == d0) && d0 >= 0) wdoc = d0;
+      }
       for (bool first = true; c != kNoChunk; first = false, ++n) {
         const int k0 = c * kKeys, pb = n & 1, st = n % kStages;
         // per 32-key group, warp-uniform: 0 nobody sees a key, 1 some are masked, 2 all are seen
         int gk[2];
         bool dead = k0 + kKeys > lk;  // the chunk holds keys that nobody may see
-        bool same[2] = {true, true};
-        const int kd[2] = {kid[0], kid[1]};
+        bool same = true, other = false;  // the chunk is all of the rows' document, or of another one
+        if constexpr (DOCS) {
+          if (!warp_wait(smem_u32(&S.vfull[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
+          const int2 about = S.about[st];
+          same = about.x == wdoc;
+          dead = dead || about.y != 0;
+          other = about.x != kMixed && wdoc != kMixedRows && !same;
+        }
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const int k_lo = k0 + 32 * g, k_hi = k_lo + 31;
-          const bool none = k_lo >= lk || ((k_hi < pw - a.left || k_lo > pz + a.right) && k_lo >= s.prefix);
+          const bool none = other || k_lo >= lk || ((k_hi < pw - a.left || k_lo > pz + a.right) && k_lo >= s.prefix);
           const bool all = k_hi < lk && ((k_lo >= pz - a.left && k_hi <= pw + a.right) || k_hi < s.prefix);
           gk[g] = none ? 0 : all ? 2 : 1;
-          if constexpr (DOCS) {
-            dead = dead || __any_sync(0xffffffffu, kd[g] < 0);
-            const int d0 = __shfl_sync(0xffffffffu, qdoc, 0);
-            same[g] = __all_sync(0xffffffffu, kd[g] == d0 && qdoc == d0 && d0 >= 0);
-            if (!same[g] && gk[g] == 2) gk[g] = 1;
-          }
+          if (DOCS && !same && gk[g] == 2) gk[g] = 1;
         }
         const int c_next = ch.next<DOCS>(c, map);
-        load_ids(c_next);
         if (!warp_wait(smem_u32(&S.sfull), n & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
         tc_fence_after();
         float x[64];
@@ -496,17 +540,23 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           if (gk[g] == 1) {
-            uint32_t see = window_bits(a, s, p, k0 + 32 * g);
-            if (DOCS && !same[g]) {
-              uint32_t mine = 0;
+            if (DOCS && !same) {
+              const int mine = qdoc < 0 ? kMixedRows : qdoc;
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const int4 id = *reinterpret_cast<const int4*>(&S.ids[st][32 * g + i]);
+                x[32 * g + i] = id.x == mine ? x[32 * g + i] : -INFINITY;
+                x[32 * g + i + 1] = id.y == mine ? x[32 * g + i + 1] : -INFINITY;
+                x[32 * g + i + 2] = id.z == mine ? x[32 * g + i + 2] : -INFINITY;
+                x[32 * g + i + 3] = id.w == mine ? x[32 * g + i + 3] : -INFINITY;
+              }
+            }
+            const uint32_t see = window_bits(a, s, p, k0 + 32 * g);
+            if (__any_sync(0xffffffffu, see != ~0u)) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                mine |= __shfl_sync(0xffffffffu, kd[g], i) == qdoc ? 1u << i : 0u;
-              see = qdoc >= 0 ? see & mine : 0u;
+                if (!(see >> i & 1)) x[32 * g + i] = -INFINITY;
             }
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(see >> i & 1)) x[32 * g + i] = -INFINITY;
           }
           if (gk[g] != 0) {
 #pragma unroll
@@ -545,8 +595,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           // V rows of keys that nobody may see: zero, whatever they hold (all four warps, 16 rows each)
           if (!warp_wait(smem_u32(&S.vfull[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
           const int r0 = 16 * qw + (lane >> 1);
-          const int src = __shfl_sync(0xffffffffu, qw < 2 ? kd[0] : kd[1], r0 & 31);
-          if (k0 + r0 >= lk || (DOCS && src < 0)) {
+          if (k0 + r0 >= lk || (DOCS && S.ids[st][r0] < 0)) {
 #pragma unroll
             for (int d = 0; d < kAtoms; ++d) {
               uint4* z = reinterpret_cast<uint4*>(S.v[st][d] + r0 * 128 + (lane & 1) * 64);
