@@ -14,7 +14,7 @@
 //   warp 1      MMA issuer: S = Q K^T (128 x 64 fp32, one TMEM buffer, reformed as soon as the softmax
 //               warps have copied it) and O += P V (P from TMEM, V MN-major from its TMA tile)
 //   warps 2..5  softmax, one query row per thread; a unit's O / l is written during the next unit's
-//               first chunk (after it at head dim 64, where O has two buffers)
+//               first chunk (O has two buffers at head dim 64)
 // Chunks are skipped whole where the window, the prefix or the documents leave nothing; a document's
 // chunks are found once per unit from the key ids. Inside a chunk, groups of 32 keys that every row of
 // a warp sees skip the masking. The reference maximum is raised only when it grows by more than 2^8, so
@@ -50,18 +50,19 @@ struct Chunks {
     if constexpr (!DOCS) {
       if (c >= end_a) c = max(c, beg_b);
       return c < hi ? c : kNoChunk;
-    }
-    for (; c < hi; ++c) {
-      if (c >= end_a && c < beg_b) {
-        c = beg_b;
-        if (c >= hi) break;
+    } else {
+      for (; c < hi; ++c) {
+        if (c >= end_a && c < beg_b) {
+          c = beg_b;
+          if (c >= hi) break;
+        }
+        if (c >= kDocWords * 32) return c;
+        const uint32_t rest = docs[c >> 5] >> (c & 31);
+        if (rest & 1) return c;
+        if (rest == 0) c |= 31;  // on to the next word
       }
-      if (c >= kDocWords * 32) return c;
-      const uint32_t rest = docs[c >> 5] >> (c & 31);
-      if (rest & 1) return c;
-      if (rest == 0) c |= 31;  // on to the next word
+      return kNoChunk;
     }
-    return kNoChunk;
   }
 };
 
@@ -81,6 +82,7 @@ struct VarlenSmem {
   alignas(1024) uint8_t k[kStages][D / 64][kAtom];
   alignas(1024) uint8_t v[kStages][D / 64][kAtom];
   uint32_t docs[kRing][kDocWords];
+  int row_doc[kRing][kRows];  // the documents of a unit's rows; past its last row, that row's
   // per V stage: the chunk's document ids, {the one id that all its keys have or kMixed, whether it
   // holds keys that nobody may see}
   alignas(16) int ids[kStages][kKeys];
@@ -89,6 +91,7 @@ struct VarlenSmem {
   alignas(8) uint64_t ufull[kRing], uempty[kRing];
   uint64_t qfull[kQSlots], qempty[kQSlots], kfull[kStages], kempty[kStages], vfull[kStages], vempty[kStages];
   uint64_t sfull, sfree, pfull[2], pfree[2], drain;
+  uint64_t ofree;  // head dim 128: the one O buffer may take the next unit
   uint32_t tmem;
   int abort;
 };
@@ -139,6 +142,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     mbar_init(smem_u32(&S.sfull), 1);
     mbar_init(smem_u32(&S.sfree), 4);
     mbar_init(smem_u32(&S.drain), 1);
+    mbar_init(smem_u32(&S.ofree), 4);
     S.abort = 0;
     fence_mbar_init();
   }
@@ -192,7 +196,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         int lo = 0x7fffffff, hi = -1;
 #pragma unroll
         for (int i = 0; i < kRows; i += 32) {
-          const int d = lane + i < u.rows ? a.doc_q[u.q_row + lane + i] : -1;
+          const int d = a.doc_q[u.q_row + min(lane + i, u.rows - 1)];
+          S.row_doc[rs][lane + i] = d;
           lo = min(lo, d < 0 ? 0x7fffffff : d);
           hi = max(hi, d);
         }
@@ -319,12 +324,14 @@ __global__ void __launch_bounds__(kThreads, 2)
       int n = 0, nq = 0, nu = 0;
       int pend = -1;           // chunk whose product with V is still to be issued
       bool pend_first = false; // it starts its unit's O
+      int pend_unit = 0;
       uint32_t pend_o = kTmemO;
       // O += P V of the pending chunk; V's atoms of 64 columns are separate products
       auto pv = [&]() -> bool {
         const int st = pend % kStages, pb = pend & 1;
         if (!mbar_wait(smem_u32(&S.pfull[pb]), (pend >> 1) & 1, abort, err, kErrAttnMma)) return false;
         if (!mbar_wait(smem_u32(&S.vfull[st]), (pend / kStages) & 1, abort, err, kErrAttnMma)) return false;
+        if (D == 128 && pend_first && !mbar_wait(smem_u32(&S.ofree), pend_unit & 1, abort, err, kErrAttnMma)) return false;
         tc_fence_after();
 #pragma unroll
         for (int d = 0; d < kAtoms; ++d)
@@ -365,6 +372,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (pend >= 0 && !pv()) { ok = false; break; }
             pend = n;
             pend_first = is_first;
+            pend_unit = nq;
             pend_o = kTmemO + (D == 64 ? static_cast<uint32_t>(nq & 1) * 64u : 0u);
           }
           if (!ok) break;
@@ -391,56 +399,53 @@ __global__ void __launch_bounds__(kThreads, 2)
     int n = 0, nq = 0, nu = 0;
     bool ok = true;
 
-    // one thread's output row, written once its unit's last product has landed
+    // One thread's output row, written once its unit's last product has landed. The loop below has one
+    // place that writes rows: the kernel's code size counts (instruction fetches stall the softmax).
     struct Row {
       bool on;          // a unit's row is waiting
+      bool zero;        // nothing is seen: no product to wait for
       int chunk;        // its last chunk
       uint32_t o;       // its TMEM columns
       long long at;     // row in q; -1: none
       int h, sp;
       float inv, lse2;
-    } wait{false, 0, 0, 0, 0, 0, 0.f, 0.f};
-    auto put = [&](bool zero) {
+    } wait{false, false, 0, 0, 0, 0, 0, 0.f, 0.f};
+    auto flush = [&]() -> bool {
+      if (!wait.on) return true;
+      wait.on = false;
+      if (!wait.zero) {
+        if (!warp_wait(smem_u32(&S.pfree[wait.chunk & 1]), (wait.chunk >> 1) & 1, abort, err, kErrAttnSoftmax))
+          return false;
+        tc_fence_after();
+      }
+      const long long part = (static_cast<long long>(wait.sp) * a.rows_q + wait.at) * a.Hq + wait.h;
       if (wait.at >= 0) {
-        if (a.splits == 1) {
-          if (a.lse) a.lse[wait.at * a.Hq + wait.h] = wait.lse2 * kLn2;
-        } else {
-          a.part_l[(static_cast<long long>(wait.sp) * a.rows_q + wait.at) * a.Hq + wait.h] = wait.lse2;
-        }
+        if (a.splits > 1) a.part_l[part] = wait.lse2;
+        else if (a.lse) a.lse[wait.at * a.Hq + wait.h] = wait.lse2 * kLn2;
       }
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) {
         float o[32];
-        if (zero) {
+        __syncwarp();
+        if (!wait.zero) tmem_ld32(tl + wait.o + 32 * d, o);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        } else {
-          tmem_ld32(tl + wait.o + 32 * d, o);
+        for (int i = 0; i < 32; ++i) o[i] = wait.zero ? 0.f : o[i] * wait.inv;
+        if (wait.at >= 0) {
+          if (a.splits == 1) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + wait.at * a.ldo + wait.h * D) + 4 * d;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] *= wait.inv;
-        }
-        if (wait.at < 0) continue;
-        if (a.splits == 1) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + wait.at * a.ldo + wait.h * D) + 4 * d;
+            for (int j = 0; j < 4; ++j)
+              dst[j] = make_uint4(pack_pair(o[8 * j], o[8 * j + 1], kType), pack_pair(o[8 * j + 2], o[8 * j + 3], kType),
+                                  pack_pair(o[8 * j + 4], o[8 * j + 5], kType), pack_pair(o[8 * j + 6], o[8 * j + 7], kType));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(a.part_o + part * D + 32 * d);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            dst[j] = make_uint4(pack_pair(o[8 * j], o[8 * j + 1], kType), pack_pair(o[8 * j + 2], o[8 * j + 3], kType),
-                                pack_pair(o[8 * j + 4], o[8 * j + 5], kType), pack_pair(o[8 * j + 6], o[8 * j + 7], kType));
-        } else {
-          float4* dst = reinterpret_cast<float4*>(
-              a.part_o + ((static_cast<long long>(wait.sp) * a.rows_q + wait.at) * a.Hq + wait.h) * D + 32 * d);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          }
         }
       }
-    };
-    auto flush = [&]() -> bool {
-      if (!wait.on) return true;
-      wait.on = false;
-      if (!warp_wait(smem_u32(&S.pfree[wait.chunk & 1]), (wait.chunk >> 1) & 1, abort, err, kErrAttnSoftmax)) return false;
-      tc_fence_after();
-      put(false);
       tc_fence_before();
+      __syncwarp();
       return true;
     };
 
@@ -448,28 +453,22 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int rs = nu % kRing;
       if (!warp_wait(smem_u32(&S.ufull[rs]), (nu / kRing) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
       const Unit& u = S.units[rs];
-      if (u.h < 0) break;
+      const bool end = u.h < 0;
       const int rows = u.rows, lk = u.lk, h = u.h;
       const int p = u.p0 + row;               // this row's key position
       const int pw = u.p0 + qw * 32, pz = pw + 31;  // the warp's first and last
-      const long long at = row < rows ? static_cast<long long>(u.q_row) + row : -1;
+      const long long at = !end && row < rows ? static_cast<long long>(u.q_row) + row : -1;
       Sequence s;
       s.lk = lk;
       s.prefix = u.prefix;
-      const int qdoc = DOCS && at >= 0 ? a.doc_q[at] : -1;
-      const float slope = MOD && a.slopes ? a.slopes[h] / a.scale : 0.f;
+      const int qdoc = DOCS ? S.row_doc[rs][row] : -1;
+      const bool idle = qw * 32 >= rows;  // none of the warp's rows is one
+      const float slope = MOD && a.slopes && !end ? a.slopes[h] / a.scale : 0.f;
       const uint32_t* map = S.docs[rs];
       const Chunks ch = u.ch;
       const uint32_t oc = kTmemO + (D == 64 ? static_cast<uint32_t>(nq & 1) * 64u : 0u);
-      int c = u.first;
-      if (c == kNoChunk) {  // nothing is seen by any of its rows
-        if (!flush()) { ok = false; break; }
-        wait = Row{false, 0, 0, at, h, u.sp, 0.f, -INFINITY};
-        put(true);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&S.uempty[rs]));
-        continue;
-      }
+      int c = end ? kNoChunk : u.first;
+      const bool none_seen = c == kNoChunk;  // nothing is seen by any of its rows, or the end
       float m_used = -INFINITY;
       float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
       int wdoc = kMixedRows;  // the document of all the warp's rows
@@ -477,7 +476,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int d0 = __shfl_sync(0xffffffffu, qdoc, 0);
         if (__all_sync(0xffffffffu, qdoc == d0) && d0 >= 0) wdoc = d0;
       }
-      for (bool first = true; c != kNoChunk; first = false, ++n) {
+      for (bool first = true;; first = false) {
+       if (!none_seen) {
         const int k0 = c * kKeys, pb = n & 1, st = n % kStages;
         // per 32-key group, warp-uniform: 0 nobody sees a key, 1 some are masked, 2 all are seen
         int gk[2];
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const int k_lo = k0 + 32 * g, k_hi = k_lo + 31;
-          const bool none = other || k_lo >= lk || ((k_hi < pw - a.left || k_lo > pz + a.right) && k_lo >= s.prefix);
+          const bool none = idle || other || k_lo >= lk || ((k_hi < pw - a.left || k_lo > pz + a.right) && k_lo >= s.prefix);
           const bool all = k_hi < lk && ((k_lo >= pz - a.left && k_hi <= pw + a.right) || k_hi < s.prefix);
           gk[g] = none ? 0 : all ? 2 : 1;
           if (DOCS && !same && gk[g] == 2) gk[g] = 1;
@@ -539,19 +539,19 @@ __global__ void __launch_bounds__(kThreads, 2)
         float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          if (gk[g] == 1) {
+          if (__builtin_expect(gk[g] == 1, 0)) {
+            uint32_t see = window_bits(a, s, p, k0 + 32 * g);
             if (DOCS && !same) {
-              const int mine = qdoc < 0 ? kMixedRows : qdoc;
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
+              const int doc = qdoc < 0 ? kMixedRows : qdoc;
+              uint32_t mine = 0;
+#pragma unroll 1
+              for (int i = 28; i >= 0; i -= 4) {
                 const int4 id = *reinterpret_cast<const int4*>(&S.ids[st][32 * g + i]);
-                x[32 * g + i] = id.x == mine ? x[32 * g + i] : -INFINITY;
-                x[32 * g + i + 1] = id.y == mine ? x[32 * g + i + 1] : -INFINITY;
-                x[32 * g + i + 2] = id.z == mine ? x[32 * g + i + 2] : -INFINITY;
-                x[32 * g + i + 3] = id.w == mine ? x[32 * g + i + 3] : -INFINITY;
+                mine = mine << 4 | (id.x == doc ? 1u : 0u) | (id.y == doc ? 2u : 0u) | (id.z == doc ? 4u : 0u) |
+                       (id.w == doc ? 8u : 0u);
               }
+              see &= mine;
             }
-            const uint32_t see = window_bits(a, s, p, k0 + 32 * g);
             if (__any_sync(0xffffffffu, see != ~0u)) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
         }
-        if (dead) {
+        if (__builtin_expect(dead, 0)) {
           // V rows of keys that nobody may see: zero, whatever they hold (all four warps, 16 rows each)
           if (!warp_wait(smem_u32(&S.vfull[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
           const int r0 = 16 * qw + (lane >> 1);
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor core reads V
         }
         // O may be rescaled once the product in flight has landed
-        if (!first && __any_sync(0xffffffffu, resc_o)) {
+        if (__builtin_expect(!first && __any_sync(0xffffffffu, resc_o), 0)) {
           if (!warp_wait(smem_u32(&S.pfree[(n - 1) & 1]), ((n - 1) >> 1) & 1, abort, err, kErrAttnSoftmax)) {
             ok = false;
             break;
@@ -627,23 +627,26 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         tc_fence_after();
         tmem_st32u(tl + kTmemP + pb * 32, pk);
-        // with one O buffer the previous unit's O leaves before this unit's first product
-        if (D == 128 && first && !flush()) { ok = false; break; }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&S.pfull[pb]));
-        if (D == 64 && first && !flush()) { ok = false; break; }
         c = c_next;
+        ++n;
+       }
+        if (first) {  // the previous unit's rows
+          if (!flush()) { ok = false; break; }
+          if (D == 128 && !none_seen && lane == 0) mbar_arrive(smem_u32(&S.ofree));
+        }
+        if (c == kNoChunk) break;
       }
-      if (!ok) break;
+      if (!ok || end) break;
       const float l = (la.x + la.y) + (lb.x + lb.y);
       // a row that sees nothing is 0; NaN stays NaN
-      wait = Row{true, n - 1, oc, at, h, u.sp, l > 0.f ? 1.f / l : l, l == 0.f ? -INFINITY : m_used + log2f(l)};
-      ++nq;
+      wait = Row{true, none_seen, n - 1, oc, at, h, u.sp, l > 0.f ? 1.f / l : l, l == 0.f ? -INFINITY : m_used + log2f(l)};
+      if (!none_seen) ++nq;
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&S.uempty[rs]));
     }
-    if (ok) flush();
   }
   tc_fence_before();
   __syncwarp();
