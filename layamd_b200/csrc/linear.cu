@@ -22,7 +22,7 @@
 namespace laya {
 namespace {
 
-constexpr int kThreads = 192;  // TMA producer, MMA issuer, four epilogue warps
+constexpr int kThreads = 192;  // TMA producer, MMA issuer, four epilogue warps (the pair kernel has eight)
 constexpr int kSlabBytes = 128;                 // bytes of K per stage and row: one swizzle span
 constexpr uint32_t kRowBlock = 128 * kSlabBytes;  // 128 rows of a stage
 
@@ -35,6 +35,13 @@ __device__ __forceinline__ void put_chunk(uint8_t* row_base, int row, const floa
 #pragma unroll
   for (int j = 0; j < 16; ++j)
     *reinterpret_cast<float4*>(row_base + piece_at(row, j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+}
+// Columns 32 half .. of the chunk.
+__device__ __forceinline__ void put_half(uint8_t* row_base, int row, int half, const float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<float4*>(row_base + piece_at(row, 8 * half + j)) =
+        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
 }
 __device__ __forceinline__ void get8(float (&v)[8], const uint8_t* row_base, int row, int c8) {
   const float4 x = *reinterpret_cast<const float4*>(row_base + piece_at(row, 2 * c8));
@@ -83,11 +90,11 @@ __device__ __forceinline__ void drain_loads(uint64_t* full, int stages, uint32_t
 }
 
 // ------------------------------------------------------------------ CTA pairs
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 5, kPairEpiWarps = 8, kPairThreads = 32 * (2 + kPairEpiWarps);
 struct PairSmem {
   alignas(1024) uint8_t a[kPairStages][kRowBlock];
   alignas(1024) uint8_t b[kPairStages][kRowBlock];
-  alignas(1024) uint8_t stg[4][32 * 256];  // per epilogue warp: 32 rows of one column chunk
+  alignas(1024) uint8_t stg[kPairEpiWarps][32 * 256];  // per epilogue warp: 32 rows of one column chunk
   alignas(8) uint64_t full[kPairStages];
   uint64_t empty[kPairStages];
   uint64_t accf[2];
@@ -99,7 +106,7 @@ struct PairSmem {
 constexpr size_t pair_smem_bytes() { return sizeof(PairSmem) + 1024; }
 
 template <bool F8, int OW>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                        const LinearArgs p, int* err) {
   constexpr int BN = 256, kBK = F8 ? 128 : 64;
@@ -117,7 +124,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPairStages; ++s) { mbar_init(smem_u32(&S.full[s]), 1); mbar_init(smem_u32(&S.empty[s]), 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&S.accf[a]), 1); mbar_init(smem_u32(&S.acce[a]), 8); }
+    for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&S.accf[a]), 1); mbar_init(smem_u32(&S.acce[a]), 2 * kPairEpiWarps); }
     mbar_init(smem_u32(&S.drain), 1);
     S.abort = 0;
     fence_mbar_init();
@@ -188,21 +195,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    const int q = warp & 3;
-    uint8_t* stg = S.stg[q];
+    // Two warps per quarter of the accumulator's rows, each with every other chunk of 64 columns.
+    const int q = warp & 3, side = (warp - 2) >> 2;
+    uint8_t* stg = S.stg[warp - 2];
     const uint32_t acce_leader0 = mapa_shared(smem_u32(&S.acce[0]), 0);
     const uint32_t acce_leader1 = mapa_shared(smem_u32(&S.acce[1]), 0);
     const int r4 = lane >> 3, c8 = lane & 7;
-    // residual pieces: 16 rows of a chunk at a time, the next half chunk's in flight
-    Cols8<OW> res[2][4];
-    auto fetch = [&](Cols8<OW> (&r)[4], int t, int c, int half) {
-      if (t >= tiles) return;
-      const int mb = t / num_n, nb = t - (t / num_n) * num_n;
-      const int row = mb * 256 + (int)rank * 128 + q * 32 + half * 16 + r4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) load_resid<OW>(r[i], p, row + 4 * i, nb * BN + c * 64 + c8 * 8);
+    // A chunk's residual (32 rows x 64 columns a warp) is loaded as one batch when the chunk before it
+    // is done, under the wait for the accumulator; single loads kept in flight step by step were slower
+    // (a warp has few scoreboards, so that waiting for the oldest waits for newer ones too).
+    Cols8<OW> res[8];
+    struct Place {  // where this lane's first row of a chunk lies in resid
+      const char* at;
+      int row, col;
+      bool whole;  // 8 columns in one access
     };
-    if (p.resid) fetch(res[0], cid, 0, 0);
+    const long long step_bytes = 4 * p.ldr * OW;
+    auto place = [&](int t, int c) {
+      const int mb = t / num_n, nb = t - mb * num_n;
+      Place w;
+      w.row = t < tiles ? mb * 256 + (int)rank * 128 + q * 32 + r4 : p.M;
+      w.col = nb * BN + c * 64 + c8 * 8;
+      w.at = static_cast<const char*>(p.resid) + (static_cast<long long>(w.row) * p.ldr + w.col) * OW;
+      w.whole = p.vec_out && w.col + 8 <= p.N;
+      return w;
+    };
+    auto fetch = [&](Cols8<OW>& r, const Place& w, int step) {
+      if (w.whole) {
+        if (w.row + 4 * step < p.M) {
+#pragma unroll
+          for (int i = 0; i < OW / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(w.at + step * step_bytes)[i];
+        }
+      } else {
+        load_resid<OW>(r, p, w.row + 4 * step, w.col);
+      }
+    };
+    const Place first = place(cid, side);
+    if (p.resid) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) fetch(res[i], first, i);
+    }
     int local = 0;
     for (int t = cid; t < tiles; t += ncl, ++local) {
       const int acc = local & 1;
@@ -212,17 +244,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!warp_wait(smem_u32(&S.accf[acc]), (local >> 1) & 1, abort, err, kErrGemmAccFull)) break;
       tc_fence_after();
       const uint32_t tbase = tmem + acc * BN + (static_cast<uint32_t>(q * 32) << 16);
-      for (int c = 0; c < BN / 64; ++c) {
+#pragma unroll 1
+      for (int c = side; c < BN / 64; c += 2) {
         const int col = nb * BN + c * 64 + c8 * 8;
         ColParams cp;
         load_cols(cp, p, col);
-        {
-          float v[64];
-          tmem_ld64(tbase + c * 64, v);
-          __syncwarp();  // the previous chunk has been read
-          put_chunk(stg + lane * 256, lane, v);
+        __syncwarp();  // the previous chunk has been read
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float v[32];
+          tmem_ld32(tbase + c * 64 + 32 * half, v);
+          put_half(stg + lane * 256, lane, half, v);
         }
-        if (c == BN / 64 - 1) {  // the accumulator is in shared memory: the next tile may have it
+        if (c + 2 >= BN / 64) {  // this warp's part of the accumulator is in shared memory
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(acc ? acce_leader1 : acce_leader0);
@@ -230,19 +264,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (p.resid) {
-            if (half == 0) fetch(res[1], t, c, 1);
-            else if (c + 1 < BN / 64) fetch(res[0], t, c + 1, 0);
-            else fetch(res[0], t + ncl, 0, 0);
-          }
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + r4;
+          float v[8];
+          get8(v, stg + r * 256, r, c8);
+          emit8<OW>(v, p, cp, __shfl_sync(0xffffffffu, sa, r), res[i], row0 + r, col);
+        }
+        if (p.resid) {
+          const Place next = c + 2 < BN / 64 ? place(t, c + 2) : place(t + ncl, side);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = half * 16 + 4 * i + r4;
-            float v[8];
-            get8(v, stg + r * 256, r, c8);
-            emit8<OW>(v, p, cp, __shfl_sync(0xffffffffu, sa, r), res[half][i], row0 + r, col);
-          }
+          for (int i = 0; i < 8; ++i) fetch(res[i], next, i);
         }
       }
     }
@@ -436,7 +467,7 @@ cudaError_t prepare(int* clusters) {
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2, 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
   cfg.dynamicSmemBytes = pair_smem_bytes();
   int n = 0;
   e = cudaOccupancyMaxActiveClusters(&n, linear_pair_kernel<F8, OW>, &cfg);
@@ -486,7 +517,7 @@ cudaError_t launch(const LinearArgs& a, int num_sms, int pairs, int* err, cudaSt
     Maps m;
     if (!make_maps(&m, a, 128)) return cudaErrorInvalidValue;
     const int ncl = static_cast<int>(std::min<long long>(pair_tiles, pairs));
-    return launch_pdl(linear_pair_kernel<F8, OW>, dim3(2 * ncl), dim3(kThreads), pair_smem_bytes(), st, m.a, m.b, a,
+    return launch_pdl(linear_pair_kernel<F8, OW>, dim3(2 * ncl), dim3(kPairThreads), pair_smem_bytes(), st, m.a, m.b, a,
                       err);
   }
   const int nkb = (a.K + (F8 ? 127 : 63)) / (F8 ? 128 : 64);
