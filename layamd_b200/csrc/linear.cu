@@ -4,8 +4,10 @@
 //
 // Two kernels, chosen by the number of tiles (linear_launch):
 //   pair    persistent CTA pairs, 256 x 256 tiles with the 2-SM MMA, two accumulators so that a tile's
-//           epilogue runs under the next tile's products. For grids that fill the GPU; bound by the
-//           tensor cores, and by the output's bytes where K is small.
+//           epilogue (eight warps a CTA) runs under the next tile's products. For grids that fill the
+//           GPU. 16384 x 8192 x 4096: fp16 1.28 PFLOP/s (power), e4m3 with GELU 2.3 PFLOP/s, where the
+//           operands' way from L2 bounds it (64 KB a K block and pair, about 9 TB/s); with a residual
+//           the output's bytes show (52,287 x 1024 x 2624 e4m3 171 us, 202 with a bf16 residual).
 //   tile    one 128 x BN tile per cluster of S CTAs (BN 64 or 128), each CTA a slice of K. The partial
 //           sums go to shared memory and each CTA finishes 128 / S rows, reading the others' partials
 //           through the cluster in slice order: one launch, no workspace, and the same sums in every
@@ -545,7 +547,12 @@ cudaError_t linear_launch(const LinearArgs& in, int num_sms, int pair_clusters, 
   const long long es = type_size(a.out_type);
   a.vec_out = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.ldo * es) % 16 == 0 &&
               (!a.resid || ((reinterpret_cast<uintptr_t>(a.resid) & 15) == 0 && (a.ldr * es) % 16 == 0));
-  if (a.M <= kLinearFewRows) return linear_few_launch(a, num_sms, st);
+  // Up to 16 rows the register-fed kernel, until the weight is so large that the tile kernel's deep TMA
+  // ring streams it faster (device time, 1 to 16 rows: 5248 x 1024 bf16 6.6 against 11.6 us, 8192 x 8192
+  // e4m3 (64 MB) 21 against 23 us; 8192 x 8192 bf16 (128 MB) 36 against 30 us, 16384 x 16384 bf16 126
+  // against 105 us and e4m3 71 against 57 us).
+  const long long weight = static_cast<long long>(a.N) * a.K * type_size(a.ab_type);
+  if (a.M <= kLinearFewRows && weight < (96LL << 20)) return linear_few_launch(a, num_sms, st);
   if (a.ab_type == DT_E4M3)
     return a.out_type == DT_F32 ? launch<true, 4>(a, num_sms, pair_clusters, err, st)
                                 : launch<true, 2>(a, num_sms, pair_clusters, err, st);

@@ -1,0 +1,110 @@
+"""The layer operators in the order a layer uses them, on packed sequences: norm to 8 bits, the QKV product
+on those 8 bits, masked attention, the output product added to the residual stream, the norm again, and
+the MLP's two products, eagerly and replayed from one graph, against the same layer in 64 bits.
+
+Every operator's own error is held by its own tests; here the layer's inputs and outputs are bf16 and
+the 8-bit activations carry up to 2^-4 of rounding per element, so the layer is compared with the
+64-bit layer that rounds at the same places (to e4m3 with the same scales, to bf16): what is left are
+elements at a rounding border that fall the other way. Such an element moves a sum of K terms by at most
+2^-3 of one term; the bound below takes 1 % of the elements to do so, at random: an output's relative
+error is then at most 2^-3 * sqrt(0.01) of the branch's size for each of the four 8-bit products, 0.05.
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from tests.layer_helpers import attention, linear, norm  # noqa: E402
+
+BF, E4 = torch.bfloat16, torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module", autouse=True)
+def gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA GPU")
+
+
+def quant(w):
+    s = (w.abs().amax(1) / 448).clamp_min(2.0 ** -126)
+    return (w / s[:, None]).to(E4), s
+
+
+def norm8(h, w):
+    y = h / (h.pow(2).mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+    s = (y.abs().amax(1) / 448).float().double()
+    return (y / s[:, None]).float().to(E4).double() * s[:, None]
+
+
+def test_layer():
+    g = torch.Generator(device="cuda").manual_seed(0)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    lens, H, Hkv, D, d, inter = [100, 1, 333, 64], 8, 2, 64, 512, 1536
+    T = sum(lens)
+    cu = torch.tensor([0, 100, 101, 434, 498], dtype=torch.int32, device="cuda")
+    pre = torch.tensor([10, 0, 100, 64], dtype=torch.int32, device="cuda")
+    ids = torch.tensor([i // 50 for n in lens for i in range(n)], dtype=torch.int32, device="cuda")
+    x0, n1, n2 = 3 * rnd(T, d), 1 + 0.1 * rnd(d), 1 + 0.1 * rnd(d)
+    width = (H + 2 * Hkv) * D
+    (wq, sq), (wo, so) = quant(rnd(width, d) / math.sqrt(d)), quant(rnd(d, H * D) / math.sqrt(d))
+    (wi, si), (wm, sm) = quant(rnd(inter, d) / math.sqrt(d)), quant(rnd(d, inter) / math.sqrt(inter))
+    b = 0.1 * rnd(inter)
+    x = x0.clone()
+    a8, s8 = torch.empty(T, d, device="cuda", dtype=E4), torch.empty(T, device="cuda")
+    m8, ms = torch.empty(T, inter, device="cuda", dtype=E4), torch.empty(T, device="cuda")
+    qkv, att = torch.empty(T, width, device="cuda", dtype=BF), torch.empty(T, H * D, device="cuda", dtype=BF)
+    hid, one = torch.empty(T, inter, device="cuda", dtype=BF), torch.ones(max(d, inter), device="cuda")
+    o8, os_ = torch.empty(T, H * D, device="cuda", dtype=E4), torch.empty(T, device="cuda")
+    q, k, v = qkv[:, :H * D], qkv[:, H * D:(H + Hkv) * D], qkv[:, (H + Hkv) * D:]
+
+    def layer():
+        rc = [norm(x, n1, a8, scale=s8, sync=0),
+              linear(a8, wq, qkv, s8, sq, sync=0),
+              attention(q, k, v, att, None, cu, cu, max(lens), max(lens), H, Hkv, D, cap=30.0, right=0, prefix=pre,
+                        doc_q=ids, doc_k=ids, sync=0),
+              norm(att, one[:d], o8, scale=os_, sync=0),
+              linear(o8, wo, x, os_, so, resid=x, sync=0),
+              norm(x, n2, a8, scale=s8, sync=0),
+              linear(a8, wi, hid, s8, si, bias=b, act=2, sync=0),
+              norm(hid, one[:inter], m8, scale=ms, sync=0),
+              linear(m8, wm, x, ms, sm, resid=x, sync=0)]
+        assert rc == [0] * len(rc), rc
+
+    layer()
+    torch.cuda.synchronize()
+    eager = x.clone()
+
+    f = torch.float64
+    W = lambda w, s: w.double() * s.double()[:, None]  # noqa: E731
+    h = x0.double()
+    z = (norm8(h, n1) @ W(wq, sq).t()).to(BF).double()
+    o = torch.zeros(T, H, D, dtype=f, device="cuda")
+    at = 0
+    for i, n in enumerate(lens):
+        r = z[at:at + n]
+        qq, kk, vv = (t.reshape(n, -1, D) for t in (r[:, :H * D], r[:, H * D:(H + Hkv) * D], r[:, (H + Hkv) * D:]))
+        j = torch.arange(n, device="cuda")
+        see = ((j[None] <= j[:, None]) | (j[None] < int(pre[i]))) & (ids[at:at + n, None] == ids[None, at:at + n])
+        for e in range(H):
+            s = 30 * torch.tanh(qq[:, e] @ kk[:, e // (H // Hkv)].t() / math.sqrt(D) / 30)
+            o[at:at + n, e] = torch.softmax(s.masked_fill(~see, -math.inf), 1) @ vv[:, e // (H // Hkv)]
+        at += n
+    o = o.view(T, H * D).to(BF).double()
+    branch1 = norm8(o, torch.ones(H * D, device="cuda")) @ W(wo, so).t()
+    h1 = (h + branch1).float().double()
+    u = norm8(h1, n2) @ W(wi, si).t() + b.double()
+    u = (u * torch.special.ndtr(u)).to(BF).double()
+    branch2 = norm8(u, torch.ones(inter, device="cuda")) @ W(wm, sm).t()
+    ref = h1 + branch2
+    err = (eager.double() - ref).norm() / (branch1.norm() + branch2.norm())
+    assert float(err) < 0.05, float(err)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer()
+    x.copy_(x0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(x, eager)
