@@ -197,8 +197,8 @@ int laya_b200_attention(const void* qkv, void* out, int rows, int B, const int* 
 int laya_b200_watchdog_selftest(int device, int* code, long long* cycles, float* ms);
 
 /* No counterpart in the reference. Kernel errors of the kernel-level entry points on GPU `device`
- * (laya_b200_gemm, laya_b200_gemm_splitk, laya_b200_gemm_splitk_noalloc, laya_b200_attention, the
- * watchdog self-test). A kernel whose bounded wait ran out records a code in a device word (the first
+ * (laya_b200_gemm, laya_b200_gemm_splitk, laya_b200_gemm_splitk_noalloc, laya_b200_attention, the layer
+ * operators, the watchdog self-test). A kernel whose bounded wait ran out records a code in a device word (the first
  * code wins) and ends; a call with sync != 0 reports it as -100-code, but a call with sync = 0 cannot,
  * so the word keeps the code until it is read: by the next call with sync != 0 on the same word, or by
  * this function. It waits for all work on the device, reads and clears both words (the one the
@@ -276,7 +276,8 @@ int laya_b200_linear(const void* A, long long lda, const void* W, long long ldw,
  * left, right -1: unbounded (right 0 is causal); slopes [Hq] fp32, prefix [B], doc_q [rows_q] and doc_k
  * [rows_k] (both or neither) are device arrays or NULL; lse [rows_q][Hq] fp32 or NULL. A row that sees
  * nothing gets 0 and lse -infinity. q, k, v, out are LAYA_BF16 or LAYA_F16, D is 64 or 128; their rows
- * start on 16 bytes (they may be columns of one projection's rows). out may not overlap the inputs.
+ * start on 16 bytes (they may be columns of one projection's rows). scale is positive, and with a cap
+ * scale / softcap and its inverse are normal fp32 numbers. out may not overlap the inputs.
  * max_q is at least every lq (later rows of a longer sequence are left as they are); max_k only guides
  * how the work is cut. Offsets outside the arrays are cut to them. Rows of no sequence are not written.
  * Keys behind a sequence's end or of a negative document may hold anything; other keys and values are

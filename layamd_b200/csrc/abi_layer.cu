@@ -171,6 +171,7 @@ extern "C" int laya_b200_attention_varlen(const void* q, long long ldq, const vo
                                           void* stream, int sync) {
   if (!varlen_sizes_ok(B, rows_q, max_q, max_k, Hq, Hkv, D) || rows_k < 0 || rows_k > kVarlenMaxRows) return -2;
   if (!is16(type) || !(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap)) return -2;
+  if (softcap > 0.f && (!std::isnormal(scale / softcap) || !std::isnormal(softcap / scale))) return -2;
   if (left < -1 || right < -1 || (doc_q == nullptr) != (doc_k == nullptr) || ws_bytes < 0) return -2;
   if (B == 0 || rows_q == 0 || max_q == 0) return 0;
   if (!q || !out || !cu_q || !cu_k || (rows_k > 0 && (!k || !v))) return -2;

@@ -512,7 +512,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             float top = 0.f;
 #pragma unroll
             for (int i = 0; i < 64; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
-            if (__all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
+            // (a cap so small that the coefficients would overflow takes the general form)
+            if (cap_in < 1e5f && __all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
               // the polynomial in the squared score, two lanes an instruction
               const float z1 = cap_in * cap_in, k1 = -z1 / 3.f, k2 = z1 * z1 * (2.f / 15.f),
                           k3 = z1 * z1 * z1 * (-17.f / 315.f);

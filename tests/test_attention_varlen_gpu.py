@@ -166,6 +166,14 @@ def test_caps_and_slopes(D, cap, slopes):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+def test_tiny_cap(D):
+    """A cap far below the scores (every score at +-cap, all weights nearly alike), and rows of zero scores."""
+    run([200, 70], D=D, cap=1e-7)
+    run([1, 2], [300, 90], D=D, cap=1e-7)
+    run([200], D=D, cap=1e-7, amp=0.0)
+
+
+@pytest.mark.parametrize("D", [64, 128])
 def test_prefixes(D):
     """Prefixes of no, some and all keys, with windows that leave a gap behind them, and out of range."""
     lens = [200, 513, 700, 64, 1]

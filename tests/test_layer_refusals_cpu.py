@@ -92,7 +92,8 @@ def test_attention_accepts(L):
     dict(type=F32), dict(type=E4M3), dict(D=32), dict(D=96), dict(Hq=3), dict(Hkv=0), dict(Hq=2, Hkv=4),
     dict(Hq=2048, Hkv=2), dict(B=-1), dict(B=65536), dict(rows_q=-1), dict(rows_k=-1), dict(rows_q=(1 << 29) + 1),
     dict(max_q=-1), dict(max_k=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
-    dict(scale=float("inf")), dict(softcap=-1.0), dict(softcap=float("nan")), dict(left=-2), dict(right=-2),
+    dict(scale=float("inf")), dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=1e-41),
+    dict(scale=1e-30, softcap=1e15), dict(left=-2), dict(right=-2),
     dict(doc_q=None), dict(doc_k=None), dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(cu_q=None),
     dict(cu_k=None), dict(ldq=248), dict(ldq=260), dict(ldk=120), dict(ldv=129), dict(ldo=255), dict(ldo=1 << 33),
     dict(q=A + 8), dict(k=A + 2), dict(v=A + 8), dict(out=A + 4), dict(lse=A + 2), dict(cu_q=A + 1), dict(ws=A + 8),

@@ -82,7 +82,9 @@ def case(M, N, K, ab, ot, scales, bias, act, resid, seed=0):
 SIZES = [(1, 8, 16), (1, 5248, 1024), (3, 1, 1), (7, 33, 100), (16, 1024, 2624), (16, 9601, 72), (17, 64, 64),
          (17, 1, 5), (33, 100, 1000), (77, 1153, 999), (128, 128, 128), (129, 129, 129), (200, 1024, 1024),
          (512, 1024, 2624), (300, 1000, 64), (1000, 1000, 300), (1023, 2047, 515), (2048, 2304, 768),
-         (4099, 1025, 1000), (3000, 5248, 1024), (40, 16384, 200), (5000, 40, 640)]
+         (4099, 1025, 1000), (3000, 5248, 1024), (40, 16384, 200), (5000, 40, 640),
+         # a weight so large that the tile kernel takes a few rows too
+         (1, 16390, 6200), (9, 13000, 8200)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
