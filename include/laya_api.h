@@ -198,8 +198,8 @@ int laya_b200_watchdog_selftest(int device, int* code, long long* cycles, float*
 
 /* No counterpart in the reference. Kernel errors of the kernel-level entry points on GPU `device`
  * (laya_b200_gemm, laya_b200_gemm_splitk, laya_b200_gemm_splitk_noalloc, laya_b200_attention, the layer
- * operators, the watchdog self-test). A kernel whose bounded wait ran out records a code in a device word (the first
- * code wins) and ends; a call with sync != 0 reports it as -100-code, but a call with sync = 0 cannot,
+ * operators, the watchdog self-test). A kernel whose bounded wait ran out records a code in a device
+ * word (the first code wins) and ends; a call with sync != 0 reports it as -100-code, but a call with sync = 0 cannot,
  * so the word keeps the code until it is read: by the next call with sync != 0 on the same word, or by
  * this function. It waits for all work on the device, reads and clears both words (the one the
  * allocating entries share and the one in the allocation-free entry's static array) and returns the
@@ -244,7 +244,7 @@ enum { LAYA_BF16 = 0, LAYA_F16 = 1, LAYA_F32 = 2, LAYA_E4M3 = 3 };
  *   h = x + resid;  z = h - center * mean(h);  y = z / sqrt(mean(z^2) + eps) * w + b
  * center 0: root-mean-square norm, 1: LayerNorm. resid (or NULL) and x are LAYA_BF16 / F16 / F32, w
  * and b (or NULL) fp32. sum (or NULL) receives h in sum_type; it may be x or resid itself (the same
- * pointer, type and stride). y is computed from h in fp32, before h is rounded to sum_type. out_type
+ * pointer, type and stride); out overlaps no input. y is computed from h in fp32, before h is rounded to sum_type. out_type
  * LAYA_BF16 / F16 / F32: out = y. LAYA_E4M3: scale[row] = max(max|y| / 448, 2^-126) and out = y /
  * scale[row], rounded to nearest even; scale is given exactly with this type. A row with a NaN has NaN
  * in its scale. rows 0 does nothing. */
@@ -257,7 +257,7 @@ int laya_b200_norm(const void* x, int x_type, long long ldx, const void* resid, 
  * A [M][K] and W [N][K] both LAYA_BF16, LAYA_F16 or LAYA_E4M3 (ab_type), sums in fp32; a_scale [M],
  * w_scale [N] (with any ab_type; 1 where NULL) and bias [N] (or NULL) fp32. act 0 none, 1 ReLU, 2 GELU
  * (erf), 3 SiLU. out_type LAYA_BF16 / F16 / F32 is also resid's; resid (or NULL) may be out itself (the
- * same pointer and stride). Any M, N, K up to 2^24 (K >= 1; M or N 0 does nothing). Rows of A and W start
+ * same pointer and stride), and overlaps no other input. Any M, N, K up to 2^24 (K >= 1; M or N 0 does nothing). Rows of A and W start
  * on 16 bytes: their addresses and strides in bytes are multiples of 16; what storage holds past
  * column K is not used. out, resid and the vectors may have any alignment of their type. The sums'
  * order depends only on the sizes and types. */

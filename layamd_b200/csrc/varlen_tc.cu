@@ -13,12 +13,16 @@
 //               free when its scores are formed, a V stage when its product is
 //   warp 1      MMA issuer: S = Q K^T (128 x 64 fp32, one TMEM buffer, reformed as soon as the softmax
 //               warps have copied it) and O += P V (P from TMEM, V MN-major from its TMA tile)
-//   warps 2..5  softmax, one query row per thread; a unit's O / l is written during the next unit's
-//               first chunk (O has two buffers at head dim 64)
+//   warps 2..5  softmax, one query row per thread; a unit's O / l is written after the next unit's first
+//               scores, when its last product has landed (O has two buffers at head dim 64; at 128 the
+//               next unit's first product waits for the rows)
 // Chunks are skipped whole where the window, the prefix or the documents leave nothing; a document's
 // chunks are found once per unit from the key ids. Inside a chunk, groups of 32 keys that every row of
 // a warp sees skip the masking. The reference maximum is raised only when it grows by more than 2^8, so
-// O is rarely rescaled.
+// O is rarely rescaled. What bounds it is the chain of a softmax warp's own instructions per chunk (issue
+// slots 42 % busy): 926 TFLOP/s at head dim 128 (two sequences of 8192), 520 at 64 (sequences of 2048).
+// Document masks, cap / bias and type are variants of their own because every live register near the
+// limit of 168 lengthens that chain (2048-token sequences 659 us with one kernel for all, 531 so).
 //
 // A masked score is replaced, so K may hold anything there. Keys that nobody may see (behind the
 // sequence's end, or of document -1) meet P = 0 in the product, and 0 * NaN would spoil the row: their
