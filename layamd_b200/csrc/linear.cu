@@ -36,7 +36,8 @@ __device__ __forceinline__ int piece_at(int row, int j) { return (((j >> 1) | (j
 __device__ __forceinline__ void put_chunk(uint8_t* row_base, int row, const float* v) {
 #pragma unroll
   for (int j = 0; j < 16; ++j)
-    *reinterpret_cast<float4*>(row_base + piece_at(row, j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    *reinterpret_cast<float4*>(row_base + piece_at(row, j)) =
+        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
 }
 // Columns 32 half .. of the chunk.
 __device__ __forceinline__ void put_half(uint8_t* row_base, int row, int half, const float (&v)[32]) {

@@ -481,163 +481,163 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (__all_sync(0xffffffffu, qdoc == d0) && d0 >= 0) wdoc = d0;
       }
       for (bool first = true;; first = false) {
-       if (!none_seen) {
-        const int k0 = c * kKeys, pb = n & 1, st = n % kStages;
-        // per 32-key group, warp-uniform: 0 nobody sees a key, 1 some are masked, 2 all are seen
-        int gk[2];
-        bool dead = k0 + kKeys > lk;  // the chunk holds keys that nobody may see
-        bool same = true, other = false;  // the chunk is all of the rows' document, or of another one
-        if constexpr (DOCS) {
-          if (!warp_wait(smem_u32(&S.vfull[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
-          const int2 about = S.about[st];
-          same = about.x == wdoc;
-          dead = dead || about.y != 0;
-          other = about.x != kMixed && wdoc != kMixedRows && !same;
-        }
+        if (!none_seen) {
+          const int k0 = c * kKeys, pb = n & 1, st = n % kStages;
+          // per 32-key group, warp-uniform: 0 nobody sees a key, 1 some are masked, 2 all are seen
+          int gk[2];
+          bool dead = k0 + kKeys > lk;  // the chunk holds keys that nobody may see
+          bool same = true, other = false;  // the chunk is all of the rows' document, or of another one
+          if constexpr (DOCS) {
+            if (!warp_wait(smem_u32(&S.vfull[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
+            const int2 about = S.about[st];
+            same = about.x == wdoc;
+            dead = dead || about.y != 0;
+            other = about.x != kMixed && wdoc != kMixedRows && !same;
+          }
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const int k_lo = k0 + 32 * g, k_hi = k_lo + 31;
-          const bool none = idle || other || k_lo >= lk || ((k_hi < pw - a.left || k_lo > pz + a.right) && k_lo >= s.prefix);
-          const bool all = k_hi < lk && ((k_lo >= pz - a.left && k_hi <= pw + a.right) || k_hi < s.prefix);
-          gk[g] = none ? 0 : all ? 2 : 1;
-          if (DOCS && !same && gk[g] == 2) gk[g] = 1;
-        }
-        const int c_next = ch.next<DOCS>(c, map);
-        if (!warp_wait(smem_u32(&S.sfull), n & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
-        tc_fence_after();
-        float x[64];
-        tmem_ld64(tl + kTmemS, x);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&S.sfree));  // S may take the next chunk
+          for (int g = 0; g < 2; ++g) {
+            const int k_lo = k0 + 32 * g, k_hi = k_lo + 31;
+            const bool none = idle || other || k_lo >= lk || ((k_hi < pw - a.left || k_lo > pz + a.right) && k_lo >= s.prefix);
+            const bool all = k_hi < lk && ((k_lo >= pz - a.left && k_hi <= pw + a.right) || k_hi < s.prefix);
+            gk[g] = none ? 0 : all ? 2 : 1;
+            if (DOCS && !same && gk[g] == 2) gk[g] = 1;
+          }
+          const int c_next = ch.next<DOCS>(c, map);
+          if (!warp_wait(smem_u32(&S.sfull), n & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
+          tc_fence_after();
+          float x[64];
+          tmem_ld64(tl + kTmemS, x);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&S.sfree));  // S may take the next chunk
 
-        if constexpr (MOD) {
-          if (a.cap > 0.f) {
-            float top = 0.f;
+          if constexpr (MOD) {
+            if (a.cap > 0.f) {
+              float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 64; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
-            // (a cap so small that the coefficients would overflow takes the general form)
-            if (cap_in < 1e5f && __all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
-              // the polynomial in the squared score, two lanes an instruction
-              const float z1 = cap_in * cap_in, k1 = -z1 / 3.f, k2 = z1 * z1 * (2.f / 15.f),
-                          k3 = z1 * z1 * z1 * (-17.f / 315.f);
-              const float2 c1 = make_float2(k1, k1), c2 = make_float2(k2, k2), c3 = make_float2(k3, k3),
-                           one = make_float2(1.f, 1.f);
+              for (int i = 0; i < 64; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
+              // (a cap so small that the coefficients would overflow takes the general form)
+              if (cap_in < 1e5f && __all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
+                // the polynomial in the squared score, two lanes an instruction
+                const float z1 = cap_in * cap_in, k1 = -z1 / 3.f, k2 = z1 * z1 * (2.f / 15.f),
+                            k3 = z1 * z1 * z1 * (-17.f / 315.f);
+                const float2 c1 = make_float2(k1, k1), c2 = make_float2(k2, k2), c3 = make_float2(k3, k3),
+                             one = make_float2(1.f, 1.f);
 #pragma unroll
-              for (int i = 0; i < 64; i += 2) {
-                const float2 v = make_float2(x[i], x[i + 1]), z = __fmul2_rn(v, v);
-                const float2 r = __fmul2_rn(v, __ffma2_rn(z, __ffma2_rn(z, __ffma2_rn(z, c3, c2), c1), one));
-                x[i] = r.x;
-                x[i + 1] = r.y;
+                for (int i = 0; i < 64; i += 2) {
+                  const float2 v = make_float2(x[i], x[i + 1]), z = __fmul2_rn(v, v);
+                  const float2 r = __fmul2_rn(v, __ffma2_rn(z, __ffma2_rn(z, __ffma2_rn(z, c3, c2), c1), one));
+                  x[i] = r.x;
+                  x[i + 1] = r.y;
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) x[i] = cap_out * tanh_any(x[i] * cap_in);
               }
+            }
+            if (a.slopes) {
+              const float away = static_cast<float>(p - k0);
+#pragma unroll
+              for (int i = 0; i < 64; ++i) x[i] = fmaf(-slope, fabsf(away - static_cast<float>(i)), x[i]);
+            }
+          }
+          float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (__builtin_expect(gk[g] == 1, 0)) {
+              uint32_t see = window_bits(a, s, p, k0 + 32 * g);
+              if (DOCS && !same) {
+                const int doc = qdoc < 0 ? kMixedRows : qdoc;
+                uint32_t mine = 0;
+#pragma unroll 1
+                for (int i = 28; i >= 0; i -= 4) {
+                  const int4 id = *reinterpret_cast<const int4*>(&S.ids[st][32 * g + i]);
+                  mine = mine << 4 | (id.x == doc ? 1u : 0u) | (id.y == doc ? 2u : 0u) | (id.z == doc ? 4u : 0u) |
+                         (id.w == doc ? 8u : 0u);
+                }
+                see &= mine;
+              }
+              if (__any_sync(0xffffffffu, see != ~0u)) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!(see >> i & 1)) x[32 * g + i] = -INFINITY;
+              }
+            }
+            if (gk[g] != 0) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) mq[(i >> 1) & 3] = max3(mq[(i >> 1) & 3], x[32 * g + i], x[32 * g + i + 1]);
+            }
+          }
+          const float mx = max3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * cs;
+          const float m_new = fmaxf(m_used, mx);
+          const bool resc = m_new > m_used + 8.f;
+          const bool resc_o = resc && m_used != -INFINITY;  // O is exactly 0 before a row's first visible key
+          float alpha = 1.f;
+          if (resc) {
+            alpha = exp2_fast(m_used - m_new);
+            la.x *= alpha; la.y *= alpha; lb.x *= alpha; lb.y *= alpha;
+            m_used = m_new;
+          }
+          const float msub = m_used == -INFINITY ? 0.f : m_used;
+          const float2 mul2 = make_float2(cs, cs), nm2 = make_float2(-msub, -msub);
+          uint32_t pk[32];
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (gk[g] == 0) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[16 * g + i] = 0u;
             } else {
 #pragma unroll
-              for (int i = 0; i < 64; ++i) x[i] = cap_out * tanh_any(x[i] * cap_in);
-            }
-          }
-          if (a.slopes) {
-            const float away = static_cast<float>(p - k0);
-#pragma unroll
-            for (int i = 0; i < 64; ++i) x[i] = fmaf(-slope, fabsf(away - static_cast<float>(i)), x[i]);
-          }
-        }
-        float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (__builtin_expect(gk[g] == 1, 0)) {
-            uint32_t see = window_bits(a, s, p, k0 + 32 * g);
-            if (DOCS && !same) {
-              const int doc = qdoc < 0 ? kMixedRows : qdoc;
-              uint32_t mine = 0;
-#pragma unroll 1
-              for (int i = 28; i >= 0; i -= 4) {
-                const int4 id = *reinterpret_cast<const int4*>(&S.ids[st][32 * g + i]);
-                mine = mine << 4 | (id.x == doc ? 1u : 0u) | (id.y == doc ? 2u : 0u) | (id.z == doc ? 4u : 0u) |
-                       (id.w == doc ? 8u : 0u);
+              for (int i = 0; i < 16; ++i) {
+                const float2 e = __ffma2_rn(make_float2(x[32 * g + 2 * i], x[32 * g + 2 * i + 1]), mul2, nm2);
+                const float2 pp = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                if (i & 1) lb = __fadd2_rn(lb, pp); else la = __fadd2_rn(la, pp);
+                pk[16 * g + i] = pack_pair(pp.x, pp.y, kType);
               }
-              see &= mine;
-            }
-            if (__any_sync(0xffffffffu, see != ~0u)) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(see >> i & 1)) x[32 * g + i] = -INFINITY;
             }
           }
-          if (gk[g] != 0) {
+          if (__builtin_expect(dead, 0)) {
+            // V rows of keys that nobody may see: zero, whatever they hold (all four warps, 16 rows each)
+            if (!warp_wait(smem_u32(&S.vfull[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
+            const int r0 = 16 * qw + (lane >> 1);
+            if (k0 + r0 >= lk || (DOCS && S.ids[st][r0] < 0)) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) mq[(i >> 1) & 3] = max3(mq[(i >> 1) & 3], x[32 * g + i], x[32 * g + i + 1]);
+              for (int d = 0; d < kAtoms; ++d) {
+                uint4* z = reinterpret_cast<uint4*>(S.v[st][d] + r0 * 128 + (lane & 1) * 64);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z[i] = make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor core reads V
           }
-        }
-        const float mx = max3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * cs;
-        const float m_new = fmaxf(m_used, mx);
-        const bool resc = m_new > m_used + 8.f;
-        const bool resc_o = resc && m_used != -INFINITY;  // O is exactly 0 before a row's first visible key
-        float alpha = 1.f;
-        if (resc) {
-          alpha = exp2_fast(m_used - m_new);
-          la.x *= alpha; la.y *= alpha; lb.x *= alpha; lb.y *= alpha;
-          m_used = m_new;
-        }
-        const float msub = m_used == -INFINITY ? 0.f : m_used;
-        const float2 mul2 = make_float2(cs, cs), nm2 = make_float2(-msub, -msub);
-        uint32_t pk[32];
+          // O may be rescaled once the product in flight has landed
+          if (__builtin_expect(!first && __any_sync(0xffffffffu, resc_o), 0)) {
+            if (!warp_wait(smem_u32(&S.pfree[(n - 1) & 1]), ((n - 1) >> 1) & 1, abort, err, kErrAttnSoftmax)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (gk[g] == 0) {
+            for (int d = 0; d < D / 32; ++d) {
+              float o[32];
+              tmem_ld32(tl + oc + 32 * d, o);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) pk[16 * g + i] = 0u;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 e = __ffma2_rn(make_float2(x[32 * g + 2 * i], x[32 * g + 2 * i + 1]), mul2, nm2);
-              const float2 pp = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-              if (i & 1) lb = __fadd2_rn(lb, pp); else la = __fadd2_rn(la, pp);
-              pk[16 * g + i] = pack_pair(pp.x, pp.y, kType);
+              for (int i = 0; i < 32; ++i) o[i] *= alpha;
+              tmem_st32(tl + oc + 32 * d, o);
             }
           }
-        }
-        if (__builtin_expect(dead, 0)) {
-          // V rows of keys that nobody may see: zero, whatever they hold (all four warps, 16 rows each)
-          if (!warp_wait(smem_u32(&S.vfull[st]), (n / kStages) & 1, abort, err, kErrAttnSoftmax)) { ok = false; break; }
-          const int r0 = 16 * qw + (lane >> 1);
-          if (k0 + r0 >= lk || (DOCS && S.ids[st][r0] < 0)) {
-#pragma unroll
-            for (int d = 0; d < kAtoms; ++d) {
-              uint4* z = reinterpret_cast<uint4*>(S.v[st][d] + r0 * 128 + (lane & 1) * 64);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) z[i] = make_uint4(0u, 0u, 0u, 0u);
-            }
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor core reads V
-        }
-        // O may be rescaled once the product in flight has landed
-        if (__builtin_expect(!first && __any_sync(0xffffffffu, resc_o), 0)) {
-          if (!warp_wait(smem_u32(&S.pfree[(n - 1) & 1]), ((n - 1) >> 1) & 1, abort, err, kErrAttnSoftmax)) {
+          if (n >= 2 && !warp_wait(smem_u32(&S.pfree[pb]), ((n >> 1) - 1) & 1, abort, err, kErrAttnSoftmax)) {
             ok = false;
             break;
           }
           tc_fence_after();
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d) {
-            float o[32];
-            tmem_ld32(tl + oc + 32 * d, o);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= alpha;
-            tmem_st32(tl + oc + 32 * d, o);
-          }
+          tmem_st32u(tl + kTmemP + pb * 32, pk);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&S.pfull[pb]));
+          c = c_next;
+          ++n;
         }
-        if (n >= 2 && !warp_wait(smem_u32(&S.pfree[pb]), ((n >> 1) - 1) & 1, abort, err, kErrAttnSoftmax)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        tmem_st32u(tl + kTmemP + pb * 32, pk);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&S.pfull[pb]));
-        c = c_next;
-        ++n;
-       }
         if (first) {  // the previous unit's rows
           if (!flush()) { ok = false; break; }
           if (D == 128 && !none_seen && lane == 0) mbar_arrive(smem_u32(&S.ofree));
