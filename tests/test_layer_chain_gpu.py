@@ -108,3 +108,71 @@ def test_layer():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(x, eager)
+
+
+def test_first_call_inside_a_capture_is_refused():
+    """In a fresh process: set-up is not done inside a capture (-8), the capture stays usable, and after one
+    call outside it the same capture works."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch
+from tests.layer_helpers import norm
+x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+out, y = torch.zeros_like(x), torch.zeros_like(x)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y.add_(1)
+    rc = norm(x, w, out, sync=0)
+assert rc == -8, rc
+g.replay()
+torch.cuda.synchronize()
+assert bool((y == 1).all()) and bool((out == 0).all())
+assert norm(x, w, out) == 0
+want = out.clone()
+out.zero_()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    assert norm(x, w, out, sync=0) == 0
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, want)
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_threads_at_once():
+    """Calls from several host threads, each on a stream of its own."""
+    import threading
+    g = torch.Generator(device="cuda").manual_seed(1)
+    A = torch.randn(200, 512, device="cuda", generator=g).to(BF)
+    W = torch.randn(300, 512, device="cuda", generator=g).to(BF)
+    n = torch.ones(512, device="cuda")
+    want, y = torch.empty(200, 300, device="cuda"), torch.empty(200, 512, device="cuda", dtype=BF)
+    assert norm(A, n, y) == 0 and linear(y, W, want) == 0
+    bad = []
+
+    def work():
+        torch.cuda.set_device(0)
+        s = torch.cuda.Stream()
+        mine, out = torch.empty_like(y), torch.empty_like(want)
+        s.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(s):
+            for _ in range(50):
+                if norm(A, n, mine, sync=0) or linear(mine, W, out, sync=0):
+                    bad.append("refused")
+        s.synchronize()
+        if not torch.equal(out, want):
+            bad.append("differs")
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+    from layamd_b200 import load_lib
+    assert load_lib().laya_b200_kernel_error(0) == 0
