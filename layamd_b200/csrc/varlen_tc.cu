@@ -40,7 +40,9 @@ constexpr int kDocWords = 128;  // bitmap of 4096 chunks; chunks past it are not
 constexpr uint32_t kTmemCols = 256, kTmemS = 0, kTmemO = 64, kTmemP = 192;  // P: two buffers of 32
 constexpr uint32_t kAtom = kKeys * 128;                                     // 64 rows x 128 bytes
 constexpr int kNoChunk = 0x7fffffff;
-constexpr int kMixed = -2, kMixedRows = -3;  // no single document in a chunk, in a warp's rows
+// No single document in a chunk, in a warp's rows. Every negative id of the caller's becomes -1 as it is
+// read, so that no key can have either value.
+constexpr int kMixed = -2, kMixedRows = -3;
 
 constexpr int kRing = 3;  // units published ahead
 
@@ -86,7 +88,7 @@ struct VarlenSmem {
   alignas(1024) uint8_t k[kStages][D / 64][kAtom];
   alignas(1024) uint8_t v[kStages][D / 64][kAtom];
   uint32_t docs[kRing][kDocWords];
-  int row_doc[kRing][kRows];  // the documents of a unit's rows; past its last row, that row's
+  int row_doc[kRing][kRows];  // the documents of a unit's rows (-1: none); past its last row, that row's
   // per V stage: the chunk's document ids, {the one id that all its keys have or kMixed, whether it
   // holds keys that nobody may see}
   alignas(16) int ids[kStages][kKeys];
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         int lo = 0x7fffffff, hi = -1;
 #pragma unroll
         for (int i = 0; i < kRows; i += 32) {
-          const int d = a.doc_q[u.q_row + min(lane + i, u.rows - 1)];
+          const int d = max(a.doc_q[u.q_row + min(lane + i, u.rows - 1)], -1);
           S.row_doc[rs][lane + i] = d;
           lo = min(lo, d < 0 ? 0x7fffffff : d);
           hi = max(hi, d);
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const int k = chunk * kKeys + 32 * g + lane;
-            id[g] = k < u.lk ? a.doc_k[u.k0 + k] : -1;
+            id[g] = k < u.lk ? max(a.doc_k[u.k0 + k], -1) : -1;
           }
         };
         load_ids(c);
