@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
     // x[i][2 r + e]: row g + 8 r, key kb + 8 i + 2 t + e
     const bool full = !a.doc_k && kb + 16 <= s.lk &&
                       ((kb >= p_last - a.left && kb + 15 <= p_first + a.right) || kb + 16 <= s.prefix);
-    bool small = false;
+    bool small = false;  // every score of the warp is: the general form of tanh is skipped
     if (MOD && a.cap > 0.f) {
       float big = 0.f;
 #pragma unroll
@@ -271,10 +271,14 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
           const int off = 8 * i + 2 * t + (e & 1), key = kb + off;
           float v = x[i][e];
           if constexpr (MOD) {
-            if (a.cap > 0.f)
-              v = small ? cap_out * tanh_small(v * cap_in) : cap_out * tanh_any(v * cap_in);
-            else
+            if (a.cap > 0.f) {  // each score's form by itself: a row's bits depend on nothing else in the tile
+              const float u = v * cap_in;
+              float th = tanh_small(u);
+              if (!small && !(fabsf(u) < kTanhSmall)) th = tanh_any(u);
+              v = cap_out * th;
+            } else {
               v *= cs;
+            }
             if (a.slopes) v = fmaf(-slope[r], fabsf(static_cast<float>(pos[r] - key)), v);
           } else {
             v *= cs;

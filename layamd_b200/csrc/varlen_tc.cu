@@ -518,23 +518,34 @@ __global__ void __launch_bounds__(kThreads, 2)
               float top = 0.f;
 #pragma unroll
               for (int i = 0; i < 64; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
-              // (a cap so small that the coefficients would overflow takes the general form)
-              if (cap_in < 1e5f && __all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
-                // the polynomial in the squared score, two lanes an instruction
-                const float z1 = cap_in * cap_in, k1 = -z1 / 3.f, k2 = z1 * z1 * (2.f / 15.f),
-                            k3 = z1 * z1 * z1 * (-17.f / 315.f);
-                const float2 c1 = make_float2(k1, k1), c2 = make_float2(k2, k2), c3 = make_float2(k3, k3),
-                             one = make_float2(1.f, 1.f);
+              // The polynomial in the squared score, two lanes an instruction, where the score is small, and
+              // the general form where it is not: each score by itself, so that a row's bits depend on
+              // nothing else in the tile. A warp whose scores are all small skips the general form.
+              // (A cap so small that the coefficients would overflow takes the general form only.)
+              const bool poly = cap_in < 1e5f;
+              const float z1 = cap_in * cap_in, k1 = -z1 / 3.f, k2 = z1 * z1 * (2.f / 15.f),
+                          k3 = z1 * z1 * z1 * (-17.f / 315.f);
+              const float2 c1 = make_float2(k1, k1), c2 = make_float2(k2, k2), c3 = make_float2(k3, k3),
+                           one = make_float2(1.f, 1.f);
+              auto small2 = [&](float2 v) {
+                const float2 z = __fmul2_rn(v, v);
+                return __fmul2_rn(v, __ffma2_rn(z, __ffma2_rn(z, __ffma2_rn(z, c3, c2), c1), one));
+              };
+              if (poly && __all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) {
-                  const float2 v = make_float2(x[i], x[i + 1]), z = __fmul2_rn(v, v);
-                  const float2 r = __fmul2_rn(v, __ffma2_rn(z, __ffma2_rn(z, __ffma2_rn(z, c3, c2), c1), one));
+                  const float2 r = small2(make_float2(x[i], x[i + 1]));
                   x[i] = r.x;
                   x[i + 1] = r.y;
                 }
               } else {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) x[i] = cap_out * tanh_any(x[i] * cap_in);
+                for (int i = 0; i < 64; i += 2) {
+                  const float2 r = small2(make_float2(x[i], x[i + 1]));
+                  const float u0 = x[i] * cap_in, u1 = x[i + 1] * cap_in;
+                  x[i] = poly && fabsf(u0) < kTanhSmall ? r.x : cap_out * tanh_any(u0);
+                  x[i + 1] = poly && fabsf(u1) < kTanhSmall ? r.y : cap_out * tanh_any(u1);
+                }
               }
             }
             if (a.slopes) {

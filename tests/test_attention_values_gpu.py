@@ -1,0 +1,58 @@
+"""What the values of a laya_b200_attention_varlen call may and may not depend on: nothing outside its
+visible keys and its own row, small weights of fp16, caps of any size, values that are not finite."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from tests.layer_helpers import attention, half_step  # noqa: E402
+from tests.test_attention_varlen_gpu import BF, HF, check_sequence, gpu, offsets  # noqa: E402, F401
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lq,lk", [(100, 100), (1, 100), (3, 200), (130, 500)])
+@pytest.mark.parametrize("amp", [1.0, 4.0])
+def test_capped_rows_do_not_depend_on_what_nobody_sees(D, lq, lk, amp):
+    """Rows behind the last sequence, keys behind its end and keys of padding documents may hold anything:
+    not one bit of a capped row changes with them."""
+    g = torch.Generator(device="cuda").manual_seed(lk)
+    tail = 128
+    q, k, v = ((amp * torch.randn(n + tail, D, device="cuda", generator=g)).to(HF) for n in (lq, lk, lk))
+    dk = torch.zeros(lk + tail, dtype=torch.int32, device="cuda")
+    dk[5::7] = -1
+    dq = torch.zeros(lq + tail, dtype=torch.int32, device="cuda")
+    for docs in (False, True):
+        got = []
+        for fill in (0.0, 30.0, math.inf, math.nan):
+            for t, n in ((q, lq), (k, lk), (v, lk)):
+                t[n:] = fill
+            if docs:
+                k[:lk][dk[:lk] < 0], v[:lk][dk[:lk] < 0] = fill, fill
+            out, lse = torch.empty(lq + tail, D, device="cuda", dtype=HF), torch.empty(lq + tail, 1, device="cuda")
+            assert attention(q, k, v, out, lse, offsets([lq]), offsets([lk]), lq, lk, 1, 1, D, cap=30.0,
+                             doc_q=dq if docs else None, doc_k=dk if docs else None) == 0
+            got.append((out[:lq].clone(), lse[:lq].clone()))
+        assert bool(torch.isfinite(got[0][1]).all())
+        for o, z in got[1:]:
+            assert torch.equal(o, got[0][0]) and torch.equal(z, got[0][1])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lq", [1, 100])
+def test_a_capped_row_does_not_depend_on_its_neighbours(D, lq):
+    """The first row's scores are small beside the cap; those of the rows after it are not, or are."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    n = max(lq, 4)
+    q, k, v = (torch.randn(r, D, device="cuda", generator=g).to(HF) for r in (n, 300, 300))
+    one = []
+    for amp in (1.0, 50.0):
+        x = q.clone()
+        x[1:] = (amp * q[1:].float()).to(HF)
+        out, lse = torch.empty(n, D, device="cuda", dtype=HF), torch.empty(n, 1, device="cuda")
+        assert attention(x, k, v, out, lse, offsets([n]), offsets([300]), n, 300, 1, 1, D, cap=30.0) == 0
+        one.append((out[0].clone(), lse[0].clone()))
+        check_sequence(out.view(n, 1, D), lse, x.view(n, 1, D), k.view(300, 1, D), v.view(300, 1, D), HF, D ** -0.5, 30.0)
+    if lq > 4:  # (few rows move their reference maximum together)
+        assert torch.equal(one[0][0], one[1][0]) and torch.equal(one[0][1], one[1][1])
