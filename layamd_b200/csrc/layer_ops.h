@@ -73,14 +73,19 @@ struct VarlenArgs {
   const int* prefix;   // [B] or null
   const int *doc_q, *doc_k;  // both or neither
   int splits;          // key ranges per row; above 1 the partial results go to part_*
+  int slots;           // tile kernel: 0, or how many tile slots its units run over (set by its launcher)
   float* part_o;       // [splits][rows_q][Hq][D]
   float* part_l;       // [splits][rows_q][Hq], log2 units
 };
 constexpr int kVarlenMaxRows = 1 << 29;  // positions and window edges stay in 32 bits
 constexpr int kVarlenMaxSplits = 32;
 cudaError_t varlen_prepare_device();
-// Key ranges that varlen_launch would use if the workspace allowed them.
-int varlen_splits(int B, int max_q, int max_k, int Hq, int Hkv, int num_sms);
+// Key ranges that varlen_launch would use if the workspace allowed them. Here and below max_q is at most
+// rows_q.
+int varlen_splits(int B, int rows_q, int max_q, int max_k, int Hq, int Hkv, int num_sms);
+// Query tiles and heads that the tile kernel runs over, empty ones included.
+long long varlen_units(int B, int rows_q, int max_q, int Hq);
+constexpr long long kVarlenMaxUnits = (1LL << 31) - (1 << 20);  // 32 bits, and room for one more round
 cudaError_t varlen_launch(const VarlenArgs& a, int num_sms, int* err, cudaStream_t st);
 bool varlen_few_rows(int max_q, int Hq, int Hkv);
 cudaError_t varlen_few_prepare_device();
