@@ -40,6 +40,11 @@ constexpr int kDocWords = 128;  // bitmap of 4096 chunks; chunks past it are not
 constexpr uint32_t kTmemCols = 256, kTmemS = 0, kTmemO = 64, kTmemP = 192;  // P: two buffers of 32
 constexpr uint32_t kAtom = kKeys * 128;                                     // 64 rows x 128 bytes
 constexpr int kNoChunk = 0x7fffffff;
+// Reference maxima (in log2 units) from which a row's scores are scaled before the maximum is subtracted.
+// Below, both are one FMA: the maximum was rounded and the product is not, so the difference may be off by
+// half a unit of the maximum's last place (0.25 here), for all of the row's weights alike. Above, that would
+// leave the range of P.
+constexpr float kLargeMax = 4194304.f;
 // No single document in a chunk, in a warp's rows. Every negative id of the caller's becomes -1 as it is
 // read, so that no key can have either value.
 constexpr int kMixed = -2, kMixedRows = -3;
@@ -616,7 +621,13 @@ __global__ void __launch_bounds__(kThreads, 2)
             m_used = m_new;
           }
           const float msub = m_used == -INFINITY ? 0.f : m_used;
-          const float2 mul2 = make_float2(cs, cs), nm2 = make_float2(-msub, -msub);
+          float2 mul2 = make_float2(cs, cs);
+          const float2 nm2 = make_float2(-msub, -msub);
+          if (__builtin_expect(fabsf(msub) >= kLargeMax, 0)) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) x[i] *= cs;
+            mul2 = make_float2(1.f, 1.f);
+          }
           uint32_t pk[32];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {

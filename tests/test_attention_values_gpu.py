@@ -56,3 +56,31 @@ def test_a_capped_row_does_not_depend_on_its_neighbours(D, lq):
         check_sequence(out.view(n, 1, D), lse, x.view(n, 1, D), k.view(300, 1, D), v.view(300, 1, D), HF, D ** -0.5, 30.0)
     if lq > 4:  # (few rows move their reference maximum together)
         assert torch.equal(one[0][0], one[1][0]) and torch.equal(one[0][1], one[1][1])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lq", [1, 100])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("high", [1e3, 1e6, 1e7, 1e8, 3e9, 1e15, 1e30])
+def test_large_scores(D, lq, dtype, high):
+    """Finite scores of any size, of both signs: the largest two keys of a row share it, whatever their
+    scores' last places are worth."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    n, half = 300, min(high ** 0.5, 3e4) if dtype == HF else high ** 0.5
+    scale = high / half ** 2
+    for sign in (1.0, -1.0):
+        q, k = torch.zeros(lq, D, device="cuda", dtype=dtype), torch.zeros(n, D, device="cuda", dtype=dtype)
+        q[:, 3] = sign * half * torch.linspace(0.5, 1, lq, device="cuda")
+        k[:, 3] = sign * half * torch.linspace(0.2, 0.6, n, device="cuda")
+        k[70, 3], k[130, 3] = sign * half, sign * half
+        for other in (1.0, -1.0):  # the largest scores of the row are positive, or all scores negative
+            kk = k if other > 0 else -k
+            if other < 0:
+                kk[70, 3], kk[130, 3] = -sign * half / 8, -sign * half / 8
+            v = torch.randn(n, D, device="cuda", generator=g).to(dtype)
+            out, lse = torch.empty_like(q), torch.empty(lq, 1, device="cuda")
+            assert attention(q, kk, v, out, lse, offsets([lq]), offsets([n]), lq, n, 1, 1, D, scale=scale) == 0
+            s = scale * (q[:, 3:4].double() * kk[70, 3].double())
+            mean, mag = (v[70] + v[130].float()) / 2, (v[70].float().abs() + v[130].float().abs()) / 2
+            assert bool(((out.float() - mean).abs() <= 3 * half_step(dtype) * mag).all())
+            assert bool(((lse.double() - (s + math.log(2))).abs() <= 2 ** -21 * (s.abs() + 1)).all())
