@@ -547,20 +547,19 @@ __global__ void __launch_bounds__(kThreads, 2)
               float top = 0.f;
 #pragma unroll
               for (int i = 0; i < 64; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
-              // The polynomial in the squared score, two lanes an instruction, where the score is small, and
-              // the general form where it is not: each score by itself, so that a row's bits depend on
-              // nothing else in the tile. A warp whose scores are all small skips the general form.
-              // (A cap so small that the coefficients would overflow takes the general form only.)
-              const bool poly = cap_in < 1e5f;
-              const float z1 = cap_in * cap_in, k1 = -z1 / 3.f, k2 = z1 * z1 * (2.f / 15.f),
-                          k3 = z1 * z1 * z1 * (-17.f / 315.f);
-              const float2 c1 = make_float2(k1, k1), c2 = make_float2(k2, k2), c3 = make_float2(k3, k3),
+              // The polynomial of tanh_small, two lanes an instruction, where the score is small, and the
+              // general form where it is not: each score by itself, so that a row's bits depend on nothing
+              // else in the tile. A warp whose scores are all small skips the general form. (In the capped
+              // score u = v cap_in, not in v with the cap in the coefficients: those and v^2 leave fp32's
+              // range for large caps.)
+              const float2 c0 = make_float2(cap_in, cap_in), c1 = make_float2(-1.f / 3.f, -1.f / 3.f),
+                           c2 = make_float2(2.f / 15.f, 2.f / 15.f), c3 = make_float2(-17.f / 315.f, -17.f / 315.f),
                            one = make_float2(1.f, 1.f);
               auto small2 = [&](float2 v) {
-                const float2 z = __fmul2_rn(v, v);
+                const float2 u = __fmul2_rn(v, c0), z = __fmul2_rn(u, u);
                 return __fmul2_rn(v, __ffma2_rn(z, __ffma2_rn(z, __ffma2_rn(z, c3, c2), c1), one));
               };
-              if (poly && __all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
+              if (__all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) {
                   const float2 r = small2(make_float2(x[i], x[i + 1]));
@@ -572,8 +571,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                 for (int i = 0; i < 64; i += 2) {
                   const float2 r = small2(make_float2(x[i], x[i + 1]));
                   const float u0 = x[i] * cap_in, u1 = x[i + 1] * cap_in;
-                  x[i] = poly && fabsf(u0) < kTanhSmall ? r.x : cap_out * tanh_any(u0);
-                  x[i + 1] = poly && fabsf(u1) < kTanhSmall ? r.y : cap_out * tanh_any(u1);
+                  x[i] = fabsf(u0) < kTanhSmall ? r.x : cap_out * tanh_any(u0);
+                  x[i + 1] = fabsf(u1) < kTanhSmall ? r.y : cap_out * tanh_any(u1);
                 }
               }
             }

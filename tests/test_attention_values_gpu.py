@@ -84,3 +84,42 @@ def test_large_scores(D, lq, dtype, high):
             mean, mag = (v[70] + v[130].float()) / 2, (v[70].float().abs() + v[130].float().abs()) / 2
             assert bool(((out.float() - mean).abs() <= 3 * half_step(dtype) * mag).all())
             assert bool(((lse.double() - (s + math.log(2))).abs() <= 2 ** -21 * (s.abs() + 1)).all())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lq", [1, 100])
+@pytest.mark.parametrize("cap,amp", [(1e20, 5e9), (1e30, 1e15), (1e10, 1e5), (1e-20, 1.0)])
+def test_caps_of_any_size(D, lq, cap, amp):
+    """One key's score is far above the others' (or, with a cap below them, all are alike), whose squares
+    leave fp32's range."""
+    q, k = torch.zeros(lq, D, device="cuda", dtype=BF), torch.zeros(300, D, device="cuda", dtype=BF)
+    q[:, 3], k[:, 3] = amp, amp / 2
+    k[70, 3] = 2 * amp
+    v = torch.randn(300, D, device="cuda").to(BF)
+    out, lse = torch.empty_like(q), torch.empty(lq, 1, device="cuda")
+    assert attention(q, k, v, out, lse, offsets([lq]), offsets([300]), lq, 300, 1, 1, D, scale=0.125, cap=cap) == 0
+    if cap > 1:
+        assert torch.equal(out, v[70].expand(lq, D))
+        s = cap * torch.tanh(q[:, 3:4].double() * k[70, 3].double() * 0.125 / cap)
+        assert bool(((lse.double() - s).abs() <= 2e-6 * s).all())
+    else:
+        mean, mag = v.double().mean(0), v.double().abs().mean(0)
+        assert bool(((out.double() - mean).abs() <= 2 ** -7 * mag).all())
+        assert bool(((lse.double() - math.log(300)).abs() <= 1e-5).all())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lq", [1, 100])
+@pytest.mark.parametrize("cap", [1e4, 1e6, 1e8])
+def test_scores_near_a_large_cap(D, lq, cap):
+    """Scores of a tenth to a fifth of a large cap: lse is the largest capped score, which is off by the
+    polynomial's error at u = 0.2 (62 / 2835 u^8 = 6e-8 of it) and seven roundings of 2^-24 (u, u^2, four in
+    the polynomial's sum that count less than one together, the products with v and log2 e, lse): 5e-7."""
+    q, k = torch.zeros(lq, D, device="cuda", dtype=BF), torch.zeros(64, D, device="cuda", dtype=BF)
+    q[:, 0] = 1.0
+    k[:, 0] = (cap * torch.linspace(0.1, 0.2, 64, device="cuda")).to(BF)
+    v = torch.zeros(64, D, device="cuda", dtype=BF)
+    out, lse = torch.empty_like(q), torch.empty(lq, 1, device="cuda")
+    assert attention(q, k, v, out, lse, offsets([lq]), offsets([64]), lq, 64, 1, 1, D, scale=1.0, cap=cap) == 0
+    want = torch.logsumexp(cap * torch.tanh(k[:, 0].double() / cap), 0)
+    assert float((lse.double() - want).abs().max()) <= 5e-7 * float(want)
