@@ -7,6 +7,11 @@
 
 namespace laya {
 
+// A row's weights are 2^(s - m) against a reference m that moves only when a score passes it by more than
+// 2^(kGrow + up), to up below that score. fp16's smallest number is 2^-24, so there up is 7: a weight below
+// 2^-32 of the row's largest is lost, and none passes 2^15. bf16 has fp32's range: up is 0.
+constexpr float kGrow = 8.f, kUpF16 = 7.f;
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_fast(float x) {  // 2^-inf = 0

@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
   const int group = warp >> 2, key0 = 16 * (warp & 3);
   uint32_t q[kQ][4];
   float slope[2];
-  const float cs = a.scale * kLog2e;
+  const float cs = a.scale * kLog2e, up_by = bf ? 0.f : kUpF16;
   const float cap_in = MOD && a.cap > 0.f ? a.scale / a.cap : 0.f, cap_out = a.cap * kLog2e;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
@@ -300,13 +300,13 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       top[r] = fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]));
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      up = up || top[r] > mr[r] + 8.f;
+      up = up || top[r] - mr[r] > kGrow + up_by;
     }
-    // the reference maximum moves only when some row's grows by more than 2^8
+    // the references of all rows move when one has to
     if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float m_new = fmaxf(mr[r], top[r]);
+        const float m_new = fmaxf(mr[r], top[r] - up_by);
         const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(mr[r] - m_new);
         mr[r] = m_new;
         lr[r] *= alpha;

@@ -40,7 +40,7 @@ constexpr int kDocWords = 128;  // bitmap of 4096 chunks; chunks past it are not
 constexpr uint32_t kTmemCols = 256, kTmemS = 0, kTmemO = 64, kTmemP = 192;  // P: two buffers of 32
 constexpr uint32_t kAtom = kKeys * 128;                                     // 64 rows x 128 bytes
 constexpr int kNoChunk = 0x7fffffff;
-// Reference maxima (in log2 units) from which a row's scores are scaled before the maximum is subtracted.
+// References (in log2 units) from which a row's scores are scaled before the maximum is subtracted.
 // Below, both are one FMA: the maximum was rounded and the product is not, so the difference may be off by
 // half a unit of the maximum's last place (0.25 here), for all of the row's weights alike. Above, that would
 // leave the range of P.
@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   using Smem = VarlenSmem<D>;
   constexpr int kStages = Smem::kStages, kAtoms = D / 64, kQSlots = Smem::kQSlots;
   constexpr int kType = BF ? DT_BF16 : DT_F16;
+  constexpr float kUp = BF ? 0.f : kUpF16;
   extern __shared__ uint8_t smem_raw[];
   Smem& S = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -610,11 +611,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
           const float mx = max3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * cs;
-          const float m_new = fmaxf(m_used, mx);
-          const bool resc = m_new > m_used + 8.f;
+          const bool resc = mx - m_used > kGrow + kUp;
           const bool resc_o = resc && m_used != -INFINITY;  // O is exactly 0 before a row's first visible key
           float alpha = 1.f;
           if (resc) {
+            const float m_new = mx - kUp;
             alpha = exp2_fast(m_used - m_new);
             la.x *= alpha; la.y *= alpha; lb.x *= alpha; lb.y *= alpha;
             m_used = m_new;

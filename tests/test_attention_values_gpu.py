@@ -123,3 +123,23 @@ def test_scores_near_a_large_cap(D, lq, cap):
     assert attention(q, k, v, out, lse, offsets([lq]), offsets([64]), lq, 64, 1, 1, D, scale=1.0, cap=cap) == 0
     want = torch.logsumexp(cap * torch.tanh(k[:, 0].double() / cap), 0)
     assert float((lse.double() - want).abs().max()) <= 5e-7 * float(want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lq", [1, 100])
+def test_many_small_weights_of_fp16_count(D, lq):
+    """131,071 keys of weight e^-17.75 = 2^-25.6 each beside one of weight 1: together 0.26 % of the row, each
+    below half of fp16's smallest number. A weight may be off by 2^-32 of the largest (half of that number,
+    with the weights held 2^7 up), so the output by n 2^-32 and half a step of its own."""
+    n = 1 << 17
+    q, k = torch.zeros(lq, D, device="cuda", dtype=HF), torch.zeros(n, D, device="cuda", dtype=HF)
+    v = torch.ones(n, D, device="cuda", dtype=HF)
+    q[:, 0], k[0, 0], v[0] = 4.4375, 4.0, 0.0
+    out, lse = torch.empty_like(q), torch.empty(lq, 1, device="cuda")
+    assert attention(q, k, v, out, lse, offsets([lq]), offsets([n]), lq, n, 1, 1, D, scale=1.0) == 0
+    w = (n - 1) * math.exp(-17.75)
+    want = w / (1 + w)
+    bound = n * 2.0 ** -32 + (half_step(HF) + 1e-5) * want + 2.0 ** -25
+    assert float((out.double() - want).abs().max()) <= bound
+    # (a sum of n positive fp32 terms)
+    assert float((lse.double() - (17.75 + math.log1p(w))).abs().max()) <= n * 2.0 ** -24 + 17.75 * 2.0 ** -20
