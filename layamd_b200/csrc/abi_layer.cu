@@ -144,6 +144,11 @@ namespace {
 // Bytes of the partial results of one key range.
 long long varlen_range_bytes(long long rows_q, int Hq, int D) { return rows_q * Hq * (D + 1LL) * 4; }
 
+// Key ranges that a call of these sizes is cut into: the call's own plan and the workspace query's.
+int plan_splits(int B, int rows_q, int max_q, int max_k, int Hq, int Hkv, int sms) {
+  return varlen_splits(B, rows_q, std::min(max_q, rows_q), max_k, Hq, Hkv, sms);
+}
+
 bool varlen_sizes_ok(int B, int rows_q, int max_q, int max_k, int Hq, int Hkv, int D) {
   return B >= 0 && B <= 65535 && rows_q >= 0 && rows_q <= kVarlenMaxRows && max_q >= 0 && max_q <= kVarlenMaxRows &&
          max_k >= 0 && max_k <= kVarlenMaxRows && Hkv >= 1 && Hq >= Hkv && Hq <= 1024 && Hq % Hkv == 0 &&
@@ -159,7 +164,7 @@ extern "C" long long laya_b200_attention_varlen_ws(int B, int rows_q, int max_q,
     cudaGetLastError();
     return -1;
   }
-  const int splits = varlen_splits(B, rows_q, max_q, max_k, Hq, Hkv, sms);
+  const int splits = plan_splits(B, rows_q, max_q, max_k, Hq, Hkv, sms);
   return splits > 1 ? splits * varlen_range_bytes(rows_q, Hq, D) : 0;
 }
 
@@ -223,7 +228,7 @@ extern "C" int laya_b200_attention_varlen(const void* q, long long ldq, const vo
   a.doc_k = doc_k;
   const long long range = varlen_range_bytes(rows_q, Hq, D);
   const long long fit = ws ? ws_bytes / range : 0;
-  int splits = varlen_splits(B, rows_q, a.max_q, max_k, Hq, Hkv, d.sms);
+  int splits = plan_splits(B, rows_q, max_q, max_k, Hq, Hkv, d.sms);
   if (fit < splits) splits = fit > 1 ? static_cast<int>(fit) : 1;
   a.splits = splits;
   a.part_o = static_cast<float*>(ws);
