@@ -124,8 +124,8 @@ extern "C" int laya_b200_linear(const void* A, long long lda, const void* W, lon
   if (!A || !W || !out) return -2;
   const int es = type_size(ab_type), os = type_size(out_type);
   // operand rows start on 16 bytes (the tensor copies need it); one row has no stride of its own
-  if (M == 1 && lda < K) lda = (K * (long long)es + 15) / 16 * 16 / es;
-  if (N == 1 && ldw < K) ldw = (K * (long long)es + 15) / 16 * 16 / es;
+  if (M == 1) lda = (K * (long long)es + 15) / 16 * 16 / es;
+  if (N == 1) ldw = (K * (long long)es + 15) / 16 * 16 / es;
   if (lda < K || ldw < K || lda > kLinearMaxLd || ldw > kLinearMaxLd || (lda * es) % 16 != 0 || (ldw * es) % 16 != 0)
     return -2;
   if (!is_aligned(A, 16) || !is_aligned(W, 16)) return -2;
@@ -182,14 +182,8 @@ extern "C" int laya_b200_attention_varlen(const void* q, long long ldq, const vo
   if (B == 0 || rows_q == 0 || max_q == 0) return 0;
   if (!q || !out || !cu_q || !cu_k || (rows_k > 0 && (!k || !v))) return -2;
   const long long wq = (long long)Hq * D, wk = (long long)Hkv * D;
-  if (rows_q == 1) {  // one row has no stride of its own
-    if (ldq < wq) ldq = wq;
-    if (ldo < wq) ldo = wq;
-  }
-  if (rows_k <= 1) {
-    if (ldk < wk) ldk = wk;
-    if (ldv < wk) ldv = wk;
-  }
+  if (rows_q == 1) ldq = ldo = wq;  // one row has no stride of its own
+  if (rows_k <= 1) ldk = ldv = wk;
   for (long long ld : {ldq - wq, ldk - wk, ldv - wk, ldo - wq})
     if (ld < 0 || ld > kLinearMaxLd || ld % 8 != 0) return -2;  // rows start on 16 bytes
   if (!is_aligned(q, 16) || !is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(out, 16) || !is_aligned(ws, 16) ||
