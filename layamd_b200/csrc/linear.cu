@@ -514,8 +514,8 @@ cudaError_t launch_tile(const LinearArgs& a, int splits, int* err, cudaStream_t 
 template <bool F8, int OW>
 cudaError_t launch(const LinearArgs& a, int num_sms, int pairs, int* err, cudaStream_t st) {
   const long long pair_tiles = ((a.M + 255LL) / 256) * ((a.N + 255LL) / 256);
-  // Pairs once their tiles fill at least half of the pairs the GPU holds; below that a tile per
-  // cluster, its K cut until the CTAs fill the GPU.
+  // Pairs (if any are to be used) once their tiles fill at least half of the pairs the GPU holds; below
+  // that a tile per cluster, its K cut until the CTAs fill the GPU.
   if (pairs > 0 && pair_tiles * 2 >= pairs) {
     Maps m;
     if (!make_maps(&m, a, 128)) return cudaErrorInvalidValue;
@@ -548,12 +548,25 @@ cudaError_t linear_launch(const LinearArgs& in, int num_sms, int pair_clusters, 
   const long long es = type_size(a.out_type);
   a.vec_out = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.ldo * es) % 16 == 0 &&
               (!a.resid || ((reinterpret_cast<uintptr_t>(a.resid) & 15) == 0 && (a.ldr * es) % 16 == 0));
-  // Up to 16 rows the register-fed kernel, until the weight is so large that the tile kernel's deep TMA
-  // ring streams it faster (device time, 1 to 16 rows: 5248 x 1024 bf16 6.6 against 11.6 us, 8192 x 8192
-  // e4m3 (64 MB) 21 against 23 us; 8192 x 8192 bf16 (128 MB) 36 against 30 us, 16384 x 16384 bf16 126
-  // against 105 us and e4m3 71 against 57 us).
+  // Up to 16 rows the register-fed kernel, but for a large weight the tile kernel (never pairs, which would
+  // compute 256 rows) where W's rows or all of A are long. Device times in us, register-fed against tile
+  // kernel (which with short A depends on where its buffers lie, hence the ranges):
+  //   1 row    bf16 5248 x 1024 6.6 and 11.6, 8192 x 8192 36 and 31-46, 16384 x 16384 127 and 133-136,
+  //            8192 x 28672 113 and 106-118, 5000 x 32768 116 and 75-84;
+  //            e4m3 16384 x 16384 70 and 76-85, 8192 x 28672 62 and 56-65, 2048 x 65536 52 and 40-47
+  //   4 rows   bf16 16384 x 8192 67 and 75-86, 16384 x 16384 128 and 94; e4m3 16384 x 16384 70 and 75-86,
+  //            5000 x 32768 62 and 41
+  //   8 rows   bf16 8192 x 4096 21 and 25, 32000 x 4096 63 and 83, 8192 x 8192 36 and 30, 16384 x 8192 66
+  //            and 52; e4m3 19200 x 8192 44 and 62, 16384 x 16384 70 and 53
+  //   16 rows  e4m3 16384 x 8192 40 and 32
+  // Against the rule stand widths just above a multiple of the GPU's CTAs (9472 x 16384 bf16 70 and 84).
   const long long weight = static_cast<long long>(a.N) * a.K * type_size(a.ab_type);
-  if (a.M <= kLinearFewRows && weight < (96LL << 20)) return linear_few_launch(a, num_sms, st);
+  if (a.M <= kLinearFewRows) {
+    const long long row = static_cast<long long>(a.K) * type_size(a.ab_type);
+    const bool tile = weight >= (96LL << 20) && (row >= 56 << 10 || a.M * row >= 128 << 10);
+    if (!tile) return linear_few_launch(a, num_sms, st);
+    pair_clusters = 0;
+  }
   if (a.ab_type == DT_E4M3)
     return a.out_type == DT_F32 ? launch<true, 4>(a, num_sms, pair_clusters, err, st)
                                 : launch<true, 2>(a, num_sms, pair_clusters, err, st);
