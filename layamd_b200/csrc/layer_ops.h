@@ -73,6 +73,16 @@ struct VarlenArgs {
   const int* prefix;   // [B] or null
   const int *doc_q, *doc_k;  // both or neither
   int splits;          // key ranges per row; above 1 the partial results go to part_*
+  // Tile kernel, set by its launcher. Scores stay in units of q.k until `to_log2` scales them for the
+  // exponential, capped ones in units of q.k / unit: a power of two, 1 unless a cap makes u = score / cap
+  // leave the middle of fp32's range.
+  struct {
+    float unit, to_log2;
+    float small;       // a capped score below this has u below kTanhSmall
+    float all_small;   // `small` where unit is 1; else below every score
+    float k1, k2, k3;  // tanh_small's coefficients for the score's square
+    float to_2u, out;  // score -> 2 u log2 e; cap
+  } caps;
   int slots;           // tile kernel: 0, or how many tile slots its units run over (set by its launcher)
   float* part_o;       // [splits][rows_q][Hq][D]
   float* part_l;       // [splits][rows_q][Hq], log2 units

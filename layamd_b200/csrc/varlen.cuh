@@ -20,6 +20,12 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2^-inf = 0
   return y;
 }
 
+__device__ __forceinline__ float rcp_fast(float x) {  // of infinity: 0
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Rows of sequence b in q and in k / v. Offsets outside the arrays, or that run backwards, are cut to
 // the arrays, so nothing outside them is ever touched.
 struct Sequence {
@@ -53,10 +59,15 @@ __device__ __forceinline__ float tanh_small(float u) {
 }
 // tanh u = 1 - 2 / (1 + e^(2u)) everywhere, to about 2e-7 absolutely.
 __device__ __forceinline__ float tanh_any(float u) {
-  const float e = exp2_fast(u * (2.f * kLog2e));
+  return fmaf(-2.f, rcp_fast(1.f + exp2_fast(u * (2.f * kLog2e))), 1.f);
+}
+// v < limit ? below : other, both of which are computed (NaN takes the other): no branch.
+__device__ __forceinline__ float pick_below(float v, float limit, float below, float other) {
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return fmaf(-2.f, r, 1.f);
+  asm("{\n\t.reg .pred p;\n\tsetp.lt.f32 p, %1, %2;\n\tselp.f32 %0, %3, %4, p;\n\t}"
+      : "=f"(r)
+      : "f"(v), "f"(limit), "f"(below), "f"(other));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi, int type) {

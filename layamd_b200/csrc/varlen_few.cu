@@ -278,14 +278,14 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
             if (a.cap > 0.f) {  // each score's form by itself: a row's bits depend on nothing else in the tile
               const float u = v * cap_in;
               float th = tanh_small(u);
-              if (!small && !(fabsf(u) < kTanhSmall)) th = tanh_any(u);
-              v = cap_out * th;
+              if (!small) th = pick_below(fabsf(u), kTanhSmall, th, tanh_any(u));
+              v = __fmul_rn(cap_out, th);  // (rounded before the maximum is subtracted, as the maximum is)
             } else {
-              v *= cs;
+              v = __fmul_rn(v, cs);
             }
             if (a.slopes) v = fmaf(-slope[r], fabsf(static_cast<float>(pos[r] - key)), v);
           } else {
-            v *= cs;
+            v = __fmul_rn(v, cs);
           }
           if (!full) {
             bool see = key < s.lk && ((key >= pos[r] - a.left && key <= pos[r] + a.right) || key < s.prefix);

@@ -28,6 +28,7 @@
 // sequence's end, or of document -1) meet P = 0 in the product, and 0 * NaN would spoil the row: their
 // V rows are set to zero in shared memory before the product is issued.
 #include <algorithm>
+#include <cmath>
 
 #include "kernels.h"
 #include "varlen.cuh"
@@ -430,8 +431,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     // ---------------- softmax: scores stay in units of q.k until the exponential scales them
     const int qw = warp & 3, row = qw * 32 + lane;  // this thread's row; warp w owns TMEM lanes 32 (w % 4) ..
     const uint32_t tl = tmem + (static_cast<uint32_t>(qw * 32) << 16);
-    const float cs = a.scale * kLog2e;
-    const float cap_in = MOD && a.cap > 0.f ? a.scale / a.cap : 0.f, cap_out = MOD ? a.cap / a.scale : 0.f;
+    const float cs = a.caps.to_log2;
     int n = 0, nq = 0, nu = 0;
     bool ok = true;
 
@@ -499,13 +499,14 @@ __global__ void __launch_bounds__(kThreads, 2)
       s.prefix = u.prefix;
       const int qdoc = DOCS ? S.row_doc[rs][row] : -1;
       const bool idle = qw * 32 >= rows;  // none of the warp's rows is one
-      const float slope = MOD && a.slopes && !end ? a.slopes[h] / a.scale : 0.f;
+      const float slope = MOD && a.slopes && !end ? a.slopes[h] / a.scale * a.caps.unit : 0.f;
       const uint32_t* map = S.docs[rs];
       const Chunks ch = u.ch;
       const uint32_t oc = kTmemO + (D == 64 ? static_cast<uint32_t>(nq & 1) * 64u : 0u);
       int c = end ? kNoChunk : u.first;
       const bool none_seen = c == kNoChunk;  // nothing is seen by any of its rows, or the end
       float m_used = -INFINITY;
+      bool large = false;  // |m_used| >= kLargeMax
       float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
       int wdoc = kMixedRows;  // the document of all the warp's rows
       if constexpr (DOCS) {
@@ -548,19 +549,17 @@ __global__ void __launch_bounds__(kThreads, 2)
               float top = 0.f;
 #pragma unroll
               for (int i = 0; i < 64; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
-              // The polynomial of tanh_small, two lanes an instruction, where the score is small, and the
-              // general form where it is not: each score by itself, so that a row's bits depend on nothing
-              // else in the tile. A warp whose scores are all small skips the general form. (In the capped
-              // score u = v cap_in, not in v with the cap in the coefficients: those and v^2 leave fp32's
-              // range for large caps.)
-              const float2 c0 = make_float2(cap_in, cap_in), c1 = make_float2(-1.f / 3.f, -1.f / 3.f),
-                           c2 = make_float2(2.f / 15.f, 2.f / 15.f), c3 = make_float2(-17.f / 315.f, -17.f / 315.f),
-                           one = make_float2(1.f, 1.f);
+              // The odd polynomial of tanh_small with the cap in its coefficients, two lanes an instruction,
+              // where the score is small; where it is not cap (1 - 2 / (1 + e^(2u))). Each score takes its form
+              // by itself, so that a row's bits depend on nothing else in the tile; a warp whose scores are
+              // all small skips the second form.
+              const float2 c1 = make_float2(a.caps.k1, a.caps.k1), c2 = make_float2(a.caps.k2, a.caps.k2),
+                           c3 = make_float2(a.caps.k3, a.caps.k3), one = make_float2(1.f, 1.f);
               auto small2 = [&](float2 v) {
-                const float2 u = __fmul2_rn(v, c0), z = __fmul2_rn(u, u);
+                const float2 z = __fmul2_rn(v, v);
                 return __fmul2_rn(v, __ffma2_rn(z, __ffma2_rn(z, __ffma2_rn(z, c3, c2), c1), one));
               };
-              if (__all_sync(0xffffffffu, top * cap_in < kTanhSmall)) {
+              if (__all_sync(0xffffffffu, top < a.caps.all_small)) {
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) {
                   const float2 r = small2(make_float2(x[i], x[i + 1]));
@@ -568,12 +567,17 @@ __global__ void __launch_bounds__(kThreads, 2)
                   x[i + 1] = r.y;
                 }
               } else {
+                const float2 unit = make_float2(a.caps.unit, a.caps.unit),
+                             ke2 = make_float2(a.caps.to_2u, a.caps.to_2u), out = make_float2(a.caps.out, a.caps.out),
+                             back = make_float2(-2.f * a.caps.out, -2.f * a.caps.out);
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) {
-                  const float2 r = small2(make_float2(x[i], x[i + 1]));
-                  const float u0 = x[i] * cap_in, u1 = x[i + 1] * cap_in;
-                  x[i] = fabsf(u0) < kTanhSmall ? r.x : cap_out * tanh_any(u0);
-                  x[i + 1] = fabsf(u1) < kTanhSmall ? r.y : cap_out * tanh_any(u1);
+                  const float2 v = __fmul2_rn(make_float2(x[i], x[i + 1]), unit);  // exact
+                  const float2 u = __fmul2_rn(v, ke2), r = small2(v);
+                  const float2 d = __fadd2_rn(make_float2(exp2_fast(u.x), exp2_fast(u.y)), one);
+                  const float2 t = __ffma2_rn(make_float2(rcp_fast(d.x), rcp_fast(d.y)), back, out);
+                  x[i] = pick_below(fabsf(v.x), a.caps.small, r.x, t.x);
+                  x[i + 1] = pick_below(fabsf(v.y), a.caps.small, r.y, t.y);
                 }
               }
             }
@@ -610,24 +614,27 @@ __global__ void __launch_bounds__(kThreads, 2)
               for (int i = 0; i < 32; i += 2) mq[(i >> 1) & 3] = max3(mq[(i >> 1) & 3], x[32 * g + i], x[32 * g + i + 1]);
             }
           }
-          const float mx = max3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * cs;
+          const float mx = __fmul_rn(max3(mq[0], mq[1], fmaxf(mq[2], mq[3])), cs);
           const bool resc = mx - m_used > kGrow + kUp;
           const bool resc_o = resc && m_used != -INFINITY;  // O is exactly 0 before a row's first visible key
           float alpha = 1.f;
-          if (resc) {
-            const float m_new = mx - kUp;
-            alpha = exp2_fast(m_used - m_new);
-            la.x *= alpha; la.y *= alpha; lb.x *= alpha; lb.y *= alpha;
-            m_used = m_new;
+          float mul = cs;
+          if (resc || large) {
+            if (resc) {
+              const float m_new = mx - kUp;
+              alpha = exp2_fast(m_used - m_new);
+              la.x *= alpha; la.y *= alpha; lb.x *= alpha; lb.y *= alpha;
+              m_used = m_new;
+              large = fabsf(m_new) >= kLargeMax;
+            }
+            if (large) {
+              mul = 1.f;
+#pragma unroll
+              for (int i = 0; i < 64; ++i) x[i] = __fmul_rn(x[i], cs);  // rounded as mx is
+            }
           }
           const float msub = m_used == -INFINITY ? 0.f : m_used;
-          float2 mul2 = make_float2(cs, cs);
-          const float2 nm2 = make_float2(-msub, -msub);
-          if (__builtin_expect(fabsf(msub) >= kLargeMax, 0)) {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) x[i] *= cs;
-            mul2 = make_float2(1.f, 1.f);
-          }
+          const float2 mul2 = make_float2(mul, mul), nm2 = make_float2(-msub, -msub);
           uint32_t pk[32];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
@@ -761,6 +768,23 @@ Pairs pairs_of(int B, int rows_q, int max_q) {
   return 2 * all > 3 * slots ? Pairs{slots, true} : Pairs{all, false};
 }
 
+// The constants of the softmax, from the caller's scale and cap.
+void set_caps(VarlenArgs* a) {
+  const bool cap = a->cap > 0.f;
+  const float r = cap ? a->scale / a->cap : 1.f;
+  const float unit = cap && (r < 0x1p-16f || r > 0x1p16f) ? std::ldexp(1.f, std::ilogb(r)) : 1.f;
+  const float in = r / unit, z1 = in * in, out = cap ? a->cap / a->scale * unit : 0.f;
+  a->caps = {unit,
+             a->scale * kLog2e / unit,
+             kTanhSmall / in,
+             unit == 1.f ? kTanhSmall / in : -1.f,
+             -z1 / 3.f,
+             z1 * z1 * (2.f / 15.f),
+             z1 * z1 * z1 * (-17.f / 315.f),
+             in * (2.f * kLog2e),
+             out};
+}
+
 template <int D>
 cudaError_t launch(const VarlenArgs& in, int num_sms, int* err, cudaStream_t st) {
   VarlenArgs a = in;
@@ -772,6 +796,7 @@ cudaError_t launch(const VarlenArgs& in, int num_sms, int* err, cudaStream_t st)
   if (!map(&tq, a.q, a.Hq, a.rows_q, a.ldq, kRows) || !map(&tk, a.k, a.Hkv, std::max(1, a.rows_k), a.ldk, kKeys) ||
       !map(&tv, a.v, a.Hkv, std::max(1, a.rows_k), a.ldv, kKeys))
     return cudaErrorInvalidValue;
+  set_caps(&a);
   const Pairs pairs = pairs_of(a.B, a.rows_q, a.max_q);
   a.slots = pairs.slots ? static_cast<int>(pairs.n) : 0;
   const long long units = pairs.n * a.Hq * a.splits;
