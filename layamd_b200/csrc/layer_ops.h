@@ -97,7 +97,7 @@ int varlen_splits(int B, int rows_q, int max_q, int max_k, int Hq, int Hkv, int 
 long long varlen_units(int B, int rows_q, int max_q, int Hq);
 constexpr long long kVarlenMaxUnits = (1LL << 31) - (1 << 20);  // 32 bits, and room for one more round
 cudaError_t varlen_launch(const VarlenArgs& a, int num_sms, int* err, cudaStream_t st);
-bool varlen_few_rows(int max_q, int Hq, int Hkv);
+bool varlen_few_rows(int max_q);
 cudaError_t varlen_few_prepare_device();
 cudaError_t varlen_few_launch(const VarlenArgs& a, int* err, cudaStream_t st);
 

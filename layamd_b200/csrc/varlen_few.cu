@@ -424,8 +424,13 @@ cudaError_t varlen_few_prepare_device() {
   return e != cudaSuccess ? e : prepare<128>();
 }
 
-// Rows that share a key head: up to four tiles of 16 are cheaper here than one of 128 per head.
-bool varlen_few_rows(int max_q, int Hq, int Hkv) { return (long long)max_q * (Hq / Hkv) <= 64; }
+// Up to 8 queries. This kernel walks the keys once for 16 rows of a group, the tile kernel once for every
+// query head, in about the same time whatever its rows hold; so the queries count, not the heads that share
+// a key head. This kernel and the tile kernel in us, 64 sequences of 4096 keys, head dim 128, 4 query heads
+// to a key head: 4 queries 220 and 656, 8 387 and 667, 16 732 and 659; 32 heads: 4 queries 210 and 596, 8
+// 384 and 596, 12 569 and 596; one head: 8 373 and 445, 16 420 and 446, 24 696 and 470. With less to do
+// (8 sequences of 4096 keys, 4 heads): 4 queries 59 and 90, 8 93 and 90, 16 138 and 90; one head 8 84 and 54.
+bool varlen_few_rows(int max_q) { return max_q <= 8; }
 
 cudaError_t varlen_few_launch(const VarlenArgs& a, int* err, cudaStream_t st) {
   return a.D == 64 ? launch<64>(a, err, st) : launch<128>(a, err, st);

@@ -846,7 +846,7 @@ long long varlen_units(int B, int rows_q, int max_q, int Hq) { return pairs_of(B
 
 int varlen_splits(int B, int rows_q, int max_q, int max_k, int Hq, int Hkv, int num_sms) {
   // Enough CTAs for two per SM, each with 4 chunks (or 512 keys of the kernel for few rows) to walk.
-  const bool few = varlen_few_rows(max_q, Hq, Hkv);
+  const bool few = varlen_few_rows(max_q);
   const long long units = few ? (long long)B * Hkv * ((max_q * (Hq / Hkv) + 15) / 16)
                               : varlen_units(B, rows_q, max_q, Hq);
   const long long most = std::max<long long>(1, max_k / (few ? 512 : 4 * kKeys));
@@ -855,7 +855,7 @@ int varlen_splits(int B, int rows_q, int max_q, int max_k, int Hq, int Hkv, int 
 }
 
 cudaError_t varlen_launch(const VarlenArgs& a, int num_sms, int* err, cudaStream_t st) {
-  cudaError_t e = varlen_few_rows(a.max_q, a.Hq, a.Hkv) ? varlen_few_launch(a, err, st)
+  cudaError_t e = varlen_few_rows(a.max_q) ? varlen_few_launch(a, err, st)
                   : a.D == 64                           ? launch<64>(a, num_sms, err, st)
                                                         : launch<128>(a, num_sms, err, st);
   if (e != cudaSuccess || a.splits == 1) return e;
