@@ -177,6 +177,7 @@ extern "C" int laya_b200_attention_varlen(const void* q, long long ldq, const vo
                                           void* stream, int sync) {
   if (!varlen_sizes_ok(B, rows_q, max_q, max_k, Hq, Hkv, D) || rows_k < 0 || rows_k > kVarlenMaxRows) return -2;
   if (!is16(type) || !(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap)) return -2;
+  if (scale > kVarlenMaxScale || softcap > kVarlenMaxScale) return -2;
   if (softcap > 0.f && (!std::isnormal(scale / softcap) || !std::isnormal(softcap / scale))) return -2;
   if (left < -1 || right < -1 || (doc_q == nullptr) != (doc_k == nullptr) || ws_bytes < 0) return -2;
   if (B == 0 || rows_q == 0 || max_q == 0) return 0;
@@ -192,7 +193,7 @@ extern "C" int laya_b200_attention_varlen(const void* q, long long ldq, const vo
     return -2;
   Device d;
   if (int rc = begin(stream, sync, {q, k, v, out, lse, cu_q, cu_k, slopes, prefix, doc_q, doc_k, ws}, &d)) return rc;
-  VarlenArgs a;
+  VarlenArgs a = {};
   a.q = q;
   a.k = rows_k > 0 ? k : q;  // without keys nothing is read through the tensor maps, which need an address
   a.v = rows_k > 0 ? v : q;

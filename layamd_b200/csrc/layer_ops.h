@@ -88,6 +88,7 @@ struct VarlenArgs {
   float* part_l;       // [splits][rows_q][Hq], log2 units
 };
 constexpr int kVarlenMaxRows = 1 << 29;  // positions and window edges stay in 32 bits
+constexpr float kVarlenMaxScale = 0x1p126f;  // scale and cap, times 2 log2 e, stay finite
 constexpr int kVarlenMaxSplits = 32;
 cudaError_t varlen_prepare_device();
 // Key ranges that varlen_launch would use if the workspace allowed them. Here and below max_q is at most
