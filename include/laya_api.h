@@ -244,23 +244,26 @@ enum { LAYA_BF16 = 0, LAYA_F16 = 1, LAYA_F32 = 2, LAYA_E4M3 = 3 };
  *   h = x + resid;  z = h - center * mean(h);  y = z / sqrt(mean(z^2) + eps) * w + b
  * center 0: root-mean-square norm, 1: LayerNorm. resid (or NULL) and x are LAYA_BF16 / F16 / F32, w
  * and b (or NULL) fp32. sum (or NULL) receives h in sum_type; it may be x or resid itself (the same
- * pointer, type and stride); out overlaps no input. y is computed from h in fp32, before h is rounded to sum_type. out_type
- * LAYA_BF16 / F16 / F32: out = y. LAYA_E4M3: scale[row] = max(max|y| / 448, 2^-126) and out = y /
- * scale[row], rounded to nearest even; scale is given exactly with this type. A row with a NaN has NaN
- * in its scale. rows 0 does nothing. */
+ * pointer, type and stride); out overlaps no input. y is computed from h in fp32, before h is rounded
+ * to sum_type: the sums of h and z^2 have to stay in fp32's range (values of 1e19 leave it). out_type
+ * LAYA_BF16 / F16 / F32: out = y. LAYA_E4M3: scale[row] = max(max|y| / 448, 2^-126) and out = y *
+ * (1 / scale[row]), rounded to nearest even; scale is given exactly with this type. A row with a NaN
+ * has NaN in its scale. rows 0 does nothing. */
 int laya_b200_norm(const void* x, int x_type, long long ldx, const void* resid, int resid_type, long long ldr,
                    void* sum, int sum_type, long long lds, const float* w, const float* b, float eps, int center,
                    void* out, int out_type, long long ldo, float* scale, int rows, int D, void* stream, int sync);
 
-/* Matrix product with everything after it in one pass (W as torch.nn.Linear stores it):
+/* Matrix product with everything after it in one pass:
  *   out[m][n] = act(a_scale[m] * w_scale[n] * sum_k A[m][k] W[n][k] + bias[n]) + resid[m][n]
  * A [M][K] and W [N][K] both LAYA_BF16, LAYA_F16 or LAYA_E4M3 (ab_type), sums in fp32; a_scale [M],
  * w_scale [N] (with any ab_type; 1 where NULL) and bias [N] (or NULL) fp32. act 0 none, 1 ReLU, 2 GELU
- * (erf), 3 SiLU. out_type LAYA_BF16 / F16 / F32 is also resid's; resid (or NULL) may be out itself (the
- * same pointer and stride), and overlaps no other input. Any M, N, K up to 2^24 (K >= 1; M or N 0 does nothing). Rows of A and W start
- * on 16 bytes: their addresses and strides in bytes are multiples of 16; what storage holds past
- * column K is not used. out, resid and the vectors may have any alignment of their type. The sums'
- * order depends only on the sizes and types. */
+ * (erf, to 1e-6 absolutely), 3 SiLU. out_type LAYA_BF16 / F16 / F32 is also resid's; resid (or NULL) may
+ * be out itself (the same pointer and stride); out overlaps no other input. Any M, N, K up to 2^24 (K >=
+ * 1; M or N 0 does nothing). Rows of A and W start on 16 bytes: their addresses and strides in bytes are
+ * multiples of 16, so rows of torch.nn.Linear's dense weight fit where K elements are a multiple of 16
+ * bytes, and have to be copied to padded storage where not (one row alone may have any stride); what
+ * storage holds past column K is not used. out, resid and the vectors may have any alignment of their
+ * type. The sums' order depends only on the sizes and types. */
 int laya_b200_linear(const void* A, long long lda, const void* W, long long ldw, int ab_type, const float* a_scale,
                      const float* w_scale, const float* bias, int act, const void* resid, long long ldr, void* out,
                      int out_type, long long ldo, int M, int N, int K, void* stream, int sync);
@@ -276,14 +279,20 @@ int laya_b200_linear(const void* A, long long lda, const void* W, long long ldw,
  * left, right -1: unbounded (right 0 is causal); slopes [Hq] fp32, prefix [B], doc_q [rows_q] and doc_k
  * [rows_k] (both or neither) are device arrays or NULL; lse [rows_q][Hq] fp32 or NULL. A row that sees
  * nothing gets 0 and lse -infinity. q, k, v, out are LAYA_BF16 or LAYA_F16, D is 64 or 128; their rows
- * start on 16 bytes (they may be columns of one projection's rows). scale is positive, and with a cap
- * scale / softcap and its inverse are normal fp32 numbers. out may not overlap the inputs.
- * max_q is at least every lq (later rows of a longer sequence are left as they are); max_k only guides
- * how the work is cut. Offsets outside the arrays are cut to them. Rows of no sequence are not written.
- * Keys behind a sequence's end or of a negative document may hold anything; other keys and values are
- * finite, or a NaN can reach rows whose masks hide it. ws: workspace for calls with few rows over many
- * keys, 16-byte aligned, laya_b200_attention_varlen_ws bytes for the same sizes (NULL or fewer bytes:
- * the keys are cut into fewer ranges, with rounding differences); two calls in flight need two. */
+ * start on 16 bytes (they may be columns of one projection's rows; one row alone may have any stride).
+ * scale is positive, scale and softcap are at most 2^126, and with a cap scale / softcap and its inverse
+ * are normal fp32 numbers; slopes[h] / scale times the longest distance stays in fp32's range. out may not overlap the inputs. Scores and sums are fp32, capped scores to
+ * within 4e-7 of the cap; the weights are rounded to the inputs' type for the product with v.
+ * max_q is at least every lq (later rows of a longer sequence are left as they are), and may lie far
+ * above them; max_k only guides how the work is cut. What needs 2^31 or more units of work (query heads
+ * times the smaller of B * max_q / 128 and B + rows_q / 128, about) is refused. Offsets outside the arrays
+ * are cut to them; behind offsets that run backwards rows may stay unwritten. Rows of no sequence are
+ * not written. Keys behind a sequence's end or of a negative document (any negative number) may hold
+ * anything; other values are finite, or a NaN can reach rows whose masks hide it. ws: workspace for
+ * calls with few rows over many keys, 16-byte aligned, laya_b200_attention_varlen_ws bytes for the same
+ * sizes (NULL or fewer bytes: the keys are cut into fewer ranges, with rounding differences); two calls
+ * in flight need two. bf16 self-attention with D 64, Hq = Hkv and a symmetric window or none runs 10 to
+ * 40 % faster through laya_b200_attention, whose lengths are a host array. */
 int laya_b200_attention_varlen(const void* q, long long ldq, const void* k, long long ldk, const void* v,
                                long long ldv, void* out, long long ldo, float* lse, int type, const int* cu_q,
                                const int* cu_k, int B, int rows_q, int rows_k, int max_q, int max_k, int Hq, int Hkv,

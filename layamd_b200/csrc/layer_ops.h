@@ -1,4 +1,4 @@
-// Host-side launchers of the layer operators (norm.cu, linear.cu, attn_varlen.cu): one transformer
+// Host-side launchers of the layer operators (norm.cu, linear*.cu, varlen_*.cu): one transformer
 // layer's norm, matrix product and attention on caller-owned device memory, of any size and type. They
 // serve the C entries of abi_layer.cu; the engine's own pass does not use them.
 #pragma once

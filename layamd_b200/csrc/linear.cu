@@ -5,13 +5,16 @@
 // Two kernels, chosen by the number of tiles (linear_launch):
 //   pair    persistent CTA pairs, 256 x 256 tiles with the 2-SM MMA, two accumulators so that a tile's
 //           epilogue (eight warps a CTA) runs under the next tile's products. For grids that fill the
-//           GPU. 16384 x 8192 x 4096: fp16 1.28 PFLOP/s (power), e4m3 with GELU 2.3 PFLOP/s, where the
-//           operands' way from L2 bounds it (64 KB a K block and pair, about 9 TB/s); with a residual
-//           the output's bytes show (52,287 x 1024 x 2624 e4m3 171 us, 202 with a bf16 residual).
+//           GPU. 16384 x 8192 x 4096: fp16 834 us in single calls and 915 back to back (1.2 PFLOP/s; a
+//           library product without an epilogue takes 684 and 689 on the same GPU, so power is not what
+//           bounds it: W, 67 MB, is read again from L2 for every two or three row blocks), e4m3 with GELU
+//           426 us (2.6 PFLOP/s), where the operands' way from L2 counts (64 KB a K block and pair); 52,287 x
+//           1024 x 2624 e4m3 129 us, 152 with a bf16 residual, 179 on inputs that L2 does not hold.
 //   tile    one 128 x BN tile per cluster of S CTAs (BN 64 or 128), each CTA a slice of K. The partial
 //           sums go to shared memory and each CTA finishes 128 / S rows, reading the others' partials
 //           through the cluster in slice order: one launch, no workspace, and the same sums in every
-//           run. For grids that cannot fill the GPU; bound by the length of a CTA's chain of loads.
+//           run. For grids that cannot fill the GPU, and a few rows of large weights; bound by a CTA's
+//           chain of loads, products and joins.
 // Both write through shared memory: a thread reads its accumulator row out of tensor memory, and the
 // warp then walks the rows with 8 lanes each, so that the residual, the output, the column scales and
 // biases are all touched by consecutive lanes, at any alignment and any odd N. The next residual

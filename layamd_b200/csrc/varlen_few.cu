@@ -6,11 +6,12 @@
 // warp, on mma.sync m16n8k16 with ldmatrix from the swizzled tiles. The warps' partial rows (each
 // with its own running maximum and sum) are joined through shared memory in warp order.
 //
-// Single tokens of 24 sequences with up to 32,768 keys (1.8 GB of K and V), capped: 328 us, 0.84 of the
+// Single tokens of 24 sequences with up to 32,768 keys (1.8 GB of K and V), capped: 356 us, 0.77 of the
 // measured copy bandwidth. Operands loaded straight into registers, with no more than 64 KB in flight
-// per SM, took 461 us; the softmax of the eight rows that four query heads leave empty another 50 us.
+// per SM, took a third longer; the softmax of the eight rows that four query heads leave empty, 15 %.
 //
-// Masked scores are replaced. Values of keys that nobody may see are set to zero in shared memory, so
+// The softmax is fp32; its weights are rounded to the inputs' type for the product with V (their sum is
+// not), as mma.sync wants operands of one type. Masked scores are replaced. Values of keys that nobody may see are set to zero in shared memory, so
 // that nothing they hold reaches a row.
 #include "kernels.h"
 #include "varlen.cuh"

@@ -5,7 +5,8 @@
 //
 // Persistent, two CTAs per SM (192 threads, 256 TMEM columns each), so that one CTA's products run
 // under the other's exponentials; units go round the CTAs, longest tiles first (causal rows near the
-// end), heads fastest, so that the units in flight share keys in L2. Within a CTA the units run through
+// end; by sequence where lengths differ much), heads fastest, so that the units in flight share keys in
+// L2. Within a CTA the units run through
 // one pipeline across their borders:
 //   warp 0      TMA producer: finds a unit's sequence and its chunks, publishes them through a ring in
 //               shared memory, loads Q (2 slots at head dim 64) and the K and V chunks into two rings
@@ -20,13 +21,17 @@
 // chunks are found once per unit from the key ids. Inside a chunk, groups of 32 keys that every row of
 // a warp sees skip the masking. The reference maximum is raised only when it grows by more than 2^8, so
 // O is rarely rescaled. What bounds it is the chain of a softmax warp's own instructions per chunk (issue
-// slots 42 % busy): 926 TFLOP/s at head dim 128 (two sequences of 8192), 520 at 64 (sequences of 2048).
-// Document masks, cap / bias and type are variants of their own because every live register near the
-// limit of 168 lengthens that chain (2048-token sequences 659 us with one kernel for all, 531 so).
+// slots 42 % busy): 850 TFLOP/s at head dim 128 (two sequences of 8192, 1288 us), 490 at 64 (16 sequences
+// of 2048, 561 us). Document masks, cap / bias and type are variants of their own because every live
+// register near the limit of 168 lengthens that chain (one kernel for all took a quarter longer there).
+//
+// The softmax is fp32; its weights are rounded to the inputs' type for the product with V (their sum is
+// not), the only form in which the tensor core takes them. A row's bits depend on its own visible keys
+// and on where they lie in the chunks, on nothing else in the tile.
 //
 // A masked score is replaced, so K may hold anything there. Keys that nobody may see (behind the
-// sequence's end, or of document -1) meet P = 0 in the product, and 0 * NaN would spoil the row: their
-// V rows are set to zero in shared memory before the product is issued.
+// sequence's end, or of a negative document) meet P = 0 in the product, and 0 * NaN would spoil the row:
+// their V rows are set to zero in shared memory before the product is issued.
 #include <algorithm>
 #include <cmath>
 
@@ -845,7 +850,7 @@ cudaError_t varlen_prepare_device() {
 long long varlen_units(int B, int rows_q, int max_q, int Hq) { return pairs_of(B, rows_q, max_q).n * Hq; }
 
 int varlen_splits(int B, int rows_q, int max_q, int max_k, int Hq, int Hkv, int num_sms) {
-  // Enough CTAs for two per SM, each with 4 chunks (or 512 keys of the kernel for few rows) to walk.
+  // Enough CTAs for two per SM, each with 4 chunks (or 512 keys of the kernel for few queries) to walk.
   const bool few = varlen_few_rows(max_q);
   const long long units = few ? (long long)B * Hkv * ((max_q * (Hq / Hkv) + 15) / 16)
                               : varlen_units(B, rows_q, max_q, Hq);
