@@ -303,12 +303,13 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
       up = up || top[r] - mr[r] > kGrow + up_by;
     }
-    // the references of all rows move when one has to
+    // a row's reference moves when its own scores pass it
     if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float m_new = fmaxf(mr[r], top[r] - up_by);
-        const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(mr[r] - m_new);
+        const bool mine = top[r] - mr[r] > kGrow + up_by;
+        const float m_new = mine ? top[r] - up_by : mr[r];
+        const float alpha = mine ? exp2_fast(mr[r] - m_new) : 1.f;
         mr[r] = m_new;
         lr[r] *= alpha;
 #pragma unroll

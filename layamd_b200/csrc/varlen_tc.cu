@@ -6,8 +6,7 @@
 // Persistent, two CTAs per SM (192 threads, 256 TMEM columns each), so that one CTA's products run
 // under the other's exponentials; units go round the CTAs, longest tiles first (causal rows near the
 // end; by sequence where lengths differ much), heads fastest, so that the units in flight share keys in
-// L2. Within a CTA the units run through
-// one pipeline across their borders:
+// L2. Within a CTA the units run through one pipeline across their borders:
 //   warp 0      TMA producer: finds a unit's sequence and its chunks, publishes them through a ring in
 //               shared memory, loads Q (2 slots at head dim 64) and the K and V chunks into two rings
 //               (4 stages at head dim 64, 2 at 128), running ahead into the next units; a K stage is
@@ -27,7 +26,7 @@
 //
 // The softmax is fp32; its weights are rounded to the inputs' type for the product with V (their sum is
 // not), the only form in which the tensor core takes them. A row's bits depend on its own visible keys
-// and on where they lie in the chunks, on nothing else in the tile.
+// and on how lengths and masks cut the work, on nothing else in the tile.
 //
 // A masked score is replaced, so K may hold anything there. Keys that nobody may see (behind the
 // sequence's end, or of a negative document) meet P = 0 in the product, and 0 * NaN would spoil the row:
