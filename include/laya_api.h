@@ -245,10 +245,10 @@ enum { LAYA_BF16 = 0, LAYA_F16 = 1, LAYA_F32 = 2, LAYA_E4M3 = 3 };
  * center 0: root-mean-square norm, 1: LayerNorm. resid (or NULL) and x are LAYA_BF16 / F16 / F32, w
  * and b (or NULL) fp32. sum (or NULL) receives h in sum_type; it may be x or resid itself (the same
  * pointer, type and stride); out overlaps no input. y is computed from h in fp32, before h is rounded
- * to sum_type: the sums of h and z^2 have to stay in fp32's range (values of 1e19 leave it). out_type
- * LAYA_BF16 / F16 / F32: out = y. LAYA_E4M3: scale[row] = max(max|y| / 448, 2^-126) and out = y *
- * (1 / scale[row]), rounded to nearest even; scale is given exactly with this type. A row with a NaN
- * has NaN in its scale. rows 0 does nothing. */
+ * to sum_type, for any h whose z stays in fp32's range (and any eps, 0 included). out_type LAYA_BF16 /
+ * F16 / F32: out = y. LAYA_E4M3: scale[row] = max(max|y| / 448, 2^-126) and out = y * (1 / scale[row]),
+ * rounded to nearest even; scale is given exactly with this type. A row with a NaN has NaN in its scale.
+ * rows 0 does nothing. */
 int laya_b200_norm(const void* x, int x_type, long long ldx, const void* resid, int resid_type, long long ldr,
                    void* sum, int sum_type, long long lds, const float* w, const float* b, float eps, int center,
                    void* out, int out_type, long long ldo, float* scale, int rows, int D, void* stream, int sync);

@@ -5,9 +5,9 @@
 // Bound by HBM: x, r and the stored sum are touched once, y once; a row stays in registers between its
 // statistics and its output. T threads own a row (T = 32, 128 or 512), each NV pieces of 8 elements, so
 // every 16-bit access is one 16-byte transaction per thread and every fp32 one two, at any alignment of
-// the rows. Statistics are
-// two-pass in fp32 (the mean first, then the squares of the differences), as the engine's LayerNorm
-// computes them; h is not rounded before them, so the stored sum's rounding never reaches y.
+// the rows. Statistics are two-pass in fp32 (the mean first, then the squares of the differences), as the
+// engine's LayerNorm computes them; h is not rounded before them, so the stored sum's rounding never
+// reaches y. A row whose squares leave fp32's range is summed again, scaled by a power of two.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -244,13 +244,41 @@ __host__ __device__ constexpr int block_threads() {
   return T < 256 ? 256 : T;
 }
 
+// Blocks per SM that the registers of the larger forms are held to: without it some take a few more than
+// fit (16-bit rows of 16384 125 us instead of 85, unaligned ones of 8191 194 instead of 135).
+template <int XW, int RW, int T, int NV, bool ALIGNED>
+constexpr int min_blocks() {
+  if (!ALIGNED) return NV != 2 ? 1 : T < 512 ? 3 : 2;
+  return NV != 4 || XW + RW > 6 ? 1 : T < 512 ? 3 : XW == 2 ? 2 : 1;
+}
+
+// Sums that fp32 does not hold: the mean's is taken times kPart (16384 elements cannot overflow it), and
+// rows whose squares leave the range are held times another power of two. Both are exact.
+constexpr float kPart = 0x1p-15f, kDown = 0x1p-80f, kUp = 0x1p96f, kTiny = 0x1p-100f;
+__device__ __forceinline__ bool lost(float sum) { return !(fabsf(sum) <= 3.402823466e38f); }
+// Whether odd(sum) holds for this thread's row, whose sum is `own`; in blocks of several rows that meet at
+// barriers (where row_sum left its partial sums in `part`), whether it holds for any of them.
+template <int T, typename F>
+__device__ __forceinline__ bool any_row(float own, const float* part, F odd) {
+  if constexpr (T == 32 || block_threads<T>() == T) return odd(own);
+  bool any = false;
+#pragma unroll
+  for (int r = 0; r < block_threads<T>() / T; ++r) {
+    float v = part[r * (T / 32)];
+#pragma unroll
+    for (int i = 1; i < T / 32; ++i) v += part[r * (T / 32) + i];
+    any = any || odd(v);
+  }
+  return any;
+}
+
 // XW / RW: sizes of x's and r's elements (RW 0: no r).
 template <int XW, int RW, int T, int NV, bool ALIGNED>
-__global__ void __launch_bounds__(block_threads<T>()) norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(block_threads<T>(), min_blocks<XW, RW, T, NV, ALIGNED>()) norm_kernel(const NormArgs a) {
   constexpr int kRows = block_threads<T>() / T;
   pdl_trigger();
   pdl_wait();
-  __shared__ float part[3][block_threads<T>() / 32];
+  __shared__ float part[4][block_threads<T>() / 32];
   const int t = threadIdx.x % T;
   const long long row = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / T;
   const bool on = row < a.rows;
@@ -288,8 +316,8 @@ __global__ void __launch_bounds__(block_threads<T>()) norm_kernel(const NormArgs
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += v[i][j];
-    const float mean = row_sum<T>(s, part[0]) / a.D;
+      for (int j = 0; j < 8; ++j) s = fmaf(v[i][j], kPart, s);
+    const float mean = row_sum<T>(s, part[0]) / (a.D * kPart);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -300,7 +328,24 @@ __global__ void __launch_bounds__(block_threads<T>()) norm_kernel(const NormArgs
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) q = fmaf(v[i][j], v[i][j], q);
-  const float rstd = 1.f / sqrtf(row_sum<T>(q, part[1]) / a.D + a.eps);
+  float squares = row_sum<T>(q, part[1]);
+  // (a sum that is too small matters only where eps does not cover it)
+  auto odd = [&](float sum) { return lost(sum) || (a.eps < kTiny && sum < kTiny); };
+  float eps = a.eps;
+  if (__builtin_expect(any_row<T>(squares, part[1], odd), 0)) {
+    const float f = lost(squares) ? kDown : odd(squares) ? kUp : 1.f;
+    eps = eps * f * f;
+    q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[i][j] *= f;
+        q = fmaf(v[i][j], v[i][j], q);
+      }
+    squares = row_sum<T>(q, part[3]);
+  }
+  const float rstd = 1.f / sqrtf(squares / a.D + eps);
 
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
